@@ -304,7 +304,7 @@ def own_attention(s):
         dq = s["dqkv"].data_ptr()
         dk = dq + 64 * c["heads"] * e
         s["grads"] = jh.attention_bias_grads(
-            s["dout"].data_ptr(), dq, dk, dk + 64 * c["kv_heads"] * e, dq_stride=stride, dkv_stride=stride,
+            s["args"], s["dout"].data_ptr(), dq, dk, dk + 64 * c["kv_heads"] * e, dq_stride=stride, dkv_stride=stride,
             dtable=pointer(s["dtable"]))
     return s
 
