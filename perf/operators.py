@@ -153,8 +153,8 @@ def work(case):
     table = 4 * BUCKETS * h if case["bias"] == "table" else 0
     if case["direction"] == "forward":
         return {"bytes": 2 * (2 * nq * d + 2 * nk * dk) + 4 * nq * h + table + 8 * nq, "flops": 4 * 64 * h * pairs(case)}
-    # read q, k, v, the outputs in 32 bits, their gradient and the log-sums; written dq, dk, dv
-    return {"bytes": 2 * (3 * nq * d + 4 * nk * dk) + 4 * nq * d + 4 * nq * h + 2 * table + 8 * nq,
+    # read q, k, v, the outputs, their gradient and the log-sums; written dq, dk, dv
+    return {"bytes": 2 * (4 * nq * d + 4 * nk * dk) + 4 * nq * h + 2 * table + 8 * nq,
             "flops": 10 * 64 * h * pairs(case)}
 
 
@@ -237,10 +237,9 @@ def prepare(case, seed):
     s["key_back"] = s["key_real"].flatten().nonzero()[:, 0]
     s["o"] = torch.empty(nq, h * 64, dtype=t, device="cuda")
     s["lse"] = torch.empty(h, nq, device="cuda")
-    s["o32"] = None
     if case["direction"] == "backward":
         o, s["lse"] = plain_forward(s)
-        s["o32"], s["o"] = o, o.to(t)
+        s["o"] = o.to(t)
         s["dout"] = (0.02 * gaussian(gen, nq, h * 64)).to(t)
         s["dqkv"] = torch.empty_like(s["qkv"])
         s["dtable"] = torch.empty_like(s["table"]) if s["table"] is not None else None
@@ -296,7 +295,7 @@ def own_attention(s):
         c["heads"], c["kv_heads"], q_stride=stride, kv_stride=stride, q_first=c["keys"] - c["rows"],
         scale=0.125, cap=c["cap"], table=pointer(s["table"]), bucket=pointer(s["bucket"]), buckets=BUCKETS,
         reach=REACH, slopes=pointer(s["slopes"]), window=c["window"], span=pointer(s["span"]),
-        lse=pointer(s["lse"]), o32=pointer(s["o32"]))
+        lse=pointer(s["lse"]))
     back = c["direction"] == "backward"
     s["scratch"] = jh.Scratch(*jh.attention_bias_scratch(s["args"], backward=back))
     if back:
@@ -423,7 +422,7 @@ def plain_backward(s):
     del sc
     q = by_head(s["q"], s["query_rows"], c["heads"], 1)
     do = by_head(s["dout"], s["query_rows"], c["heads"], 1)
-    o = by_head(s["o32"], s["query_rows"], c["heads"], 1)
+    o = by_head(s["o"], s["query_rows"], c["heads"], 1)
     v = by_head(s["v"], s["key_rows"], c["kv_heads"], each)
     ds = torch.matmul(do, v.transpose(2, 3).contiguous())
     ds = p * (ds - (do * o).sum(3, keepdim=True))
@@ -494,7 +493,7 @@ def exact(case, seed):
                 continue
             p = torch.exp(a - s["lse"].double()[x, rq][:, None]).masked_fill(~ok, 0.0)
             g = s["dout"][rq, 64 * x:64 * x + 64].double()
-            d = (g * s["o32"][rq, 64 * x:64 * x + 64].double()).sum(1, keepdim=True)
+            d = (g * s["o"][rq, 64 * x:64 * x + 64].double()).sum(1, keepdim=True)
             ds = p * (g @ v[rk, y].T - d)
             dv[rk, y] += p.T @ g
             if case["bias"] == "table":
