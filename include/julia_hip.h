@@ -187,6 +187,88 @@ int julia_hip_norm_add(const void *x, int n, int d, const float *gamma, const fl
 int julia_hip_score(const void *y, int n, int d, const void *w, float b, const uint32_t *markers,
                     int k, float *logits, void *stream, char *err, size_t err_len);
 
+/* ---- operators for encoders with relative positions, and gradients. No counterpart in the
+ * reference, whose model rotates q and k (RoPE) and which does not train. All device buffers and the
+ * stream belong to the calling thread's current device, as everywhere in this part; calls that
+ * overlap need a scratch each. */
+enum { JULIA_HIP_F16 = 0, JULIA_HIP_BF16 = 1, JULIA_HIP_F32 = 2 };
+
+/* Attention, heads of 64, f16 or bf16, whose scores may be capped, biased by distance and masked:
+ *   s_ij = scale q_i . k_j, capped (cap > 0) to cap tanh(scale q_i . k_j / cap), plus b_h(j - pos_i)
+ *   with pos_i = q_first + i, the key row that query i stands at;
+ *   o_i = sum_j exp(s_ij - lse_i) v_j, lse_i = log sum_j exp(s_ij), over the keys j that query i sees.
+ * The bias b_h(t), one of
+ *   a learned table: table[bucket[t + reach]][h], t held to [-reach, reach] (reach up to 512; `table`
+ *     is [buckets][heads] f32, `bucket` [2 reach + 1] int32, julia_hip_prep_relative_buckets; a bucket
+ *     out of range is taken to the nearest);
+ *   a slope a head: -slopes[h] |t|;
+ *   none (both null).
+ * Query i sees key j if it is in its span, [span[i][0], span[i][1]) cut to [0, nk) (null: every key;
+ * documents, prefixes, padding: julia_hip_prep_spans), and if window > 0 within |j - pos_i| <= window.
+ * A row that sees no key, or whose scores are all -inf, gets o = 0 and lse = -inf. Keys that a query
+ * does not see have no effect on it, whatever they hold.
+ * Strides are in elements between rows, multiples of 8 up to 2^22 and at least a row's width; q, k, v,
+ * o are 16-byte aligned (rows of a packed qkv do). kv_heads divides heads: query head h reads
+ * key head h / (heads / kv_heads). Scores, weights and sums are f32; weights are rounded to the
+ * type for the product with v. */
+typedef struct {
+    int type; /* JULIA_HIP_F16 or JULIA_HIP_BF16 */
+    const void *q, *k, *v;
+    int64_t q_stride, kv_stride;
+    void *o;
+    int64_t o_stride;
+    int nq, nk, heads, kv_heads, q_first;
+    float scale, cap;
+    const float *table;
+    const int32_t *bucket;
+    int buckets, reach;
+    const float *slopes;
+    int window;
+    const int32_t *span; /* [nq][2] */
+    float *lse;          /* [heads][nq], nullable: the gradients need it */
+} julia_hip_attention_bias_args;
+
+/* What the loss's gradients take: dout is its derivative by o. dq, dk, dv and dtable (with a table,
+ * [buckets][heads]; null without) are written, not added to. dk and dv hold the sums over the query
+ * heads of their key head, and over every query; the same bits at every call. */
+typedef struct {
+    const void *dout;
+    int64_t do_stride;
+    void *dq, *dk, *dv;
+    int64_t dq_stride, dkv_stride;
+    float *dtable;
+} julia_hip_attention_bias_grads;
+
+/* The scratch a call takes (backward 0: julia_hip_attention_bias; 1: the gradients'). */
+int julia_hip_attention_bias_scratch(const julia_hip_attention_bias_args *a, int backward,
+                                     size_t *ws_floats, size_t *counters, char *err, size_t err_len);
+int julia_hip_attention_bias(const julia_hip_attention_bias_args *a, const julia_hip_scratch *s,
+                             void *stream, char *err, size_t err_len);
+/* The gradients, from the arguments of the forward call and the o and lse that it left. The sums over
+ * keys and queries are f32, dtable's over every (query, key) pair from unrounded dS. What o lost when
+ * it was rounded goes into dS = P (dO V^T - dO . o). A row whose lse is past 2^20 either way (every key
+ * that it sees has a bias like the type's lowest value) takes no part. */
+int julia_hip_attention_bias_backward(const julia_hip_attention_bias_args *a,
+                                      const julia_hip_attention_bias_grads *g,
+                                      const julia_hip_scratch *s, void *stream, char *err,
+                                      size_t err_len);
+
+/* y = (x - mean) / sqrt(var + eps) . gamma + beta over rows of d values (1 to 8192) in `type`, any
+ * row stride from d on; gamma, beta (nullable) and stats ([rows][2], mean and 1 / sqrt(var + eps),
+ * nullable) f32. y may be x. */
+int julia_hip_layer_norm(int type, const void *x, int64_t x_stride, int rows, int d,
+                         const float *gamma, const float *beta, float eps, void *y,
+                         int64_t y_stride, float *stats, void *stream, char *err, size_t err_len);
+/* Its gradients: dx in `type` (may be dy or x), dgamma and dbeta (nullable) [d] f32, summed over the
+ * rows in a fixed order; all written, not added to. The scratch: julia_hip_layer_norm_scratch (no
+ * counters). */
+int julia_hip_layer_norm_backward(int type, const void *x, int64_t x_stride, const void *dy,
+                                  int64_t dy_stride, int rows, int d, const float *gamma,
+                                  const float *stats, void *dx, int64_t dx_stride, float *dgamma,
+                                  float *dbeta, const julia_hip_scratch *s, void *stream, char *err,
+                                  size_t err_len);
+int julia_hip_layer_norm_scratch(int rows, int d, size_t *ws_floats, char *err, size_t err_len);
+
 /* src/timing.rs:43-74 `timing::time` for one GEMM: `warmup` calls, then `batches` batches of
  * `per_batch` back-to-back calls between HIP events; min and median microseconds per call. */
 int julia_hip_time_gemm(const julia_hip_gemm_args *g, julia_hip_gemm_config cfg,
@@ -259,6 +341,21 @@ void julia_hip_gemm_plan_2080ti(int n, int cols, int k, int sms, int per_sm, int
                                 int *splits);
 /* The reference's per-step rule, src/gemm.rs:153-172 (choose, splits). */
 julia_hip_gemm_config julia_hip_gemm_choose_2080ti(int m, int n, int k, int sms);
+
+/* julia_hip_attention_bias's checks alone, on the host (pointers for null and alignment), and its
+ * gradients' with g not null: 0, or -1 and the reason. */
+int julia_hip_attention_bias_check(const julia_hip_attention_bias_args *a,
+                                   const julia_hip_attention_bias_grads *g, char *err, size_t err_len);
+/* The bucket of each distance t = key - query in [-reach, reach], into bucket[t + reach]. both: half of
+ * the buckets for t > 0, the others for t <= 0; else all for t <= 0 (t > 0: bucket 0). In each side the
+ * first half of the buckets hold one distance each, the others ranges whose ends grow by a constant
+ * factor and reach max_distance, past which every distance is in the last. */
+int julia_hip_prep_relative_buckets(int buckets, int max_distance, int both, int reach,
+                                    int32_t *bucket, char *err, size_t err_len);
+/* The spans of documents of lens[i] rows end to end, [sum of lens][2]: each row sees its document
+ * (prefix null), or the first prefix[i] rows of its document and those up to itself. */
+int julia_hip_prep_spans(const size_t *lens, const size_t *prefix, size_t documents, int32_t *span,
+                         char *err, size_t err_len);
 
 /* julia-rs `head::answer` (src/serve.rs:58), as the reference's tools/torch_baseline.py:214-226
  * states it for results tools/score.py compares: probabilities[i] = softmax(logits)[i] (f64);

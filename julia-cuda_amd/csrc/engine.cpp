@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "../../include/julia_hip.h"
+#include "capi.h"
 #include "kernels.h"
 #include "layer.h"
 #include "weights.h"
@@ -707,26 +708,6 @@ std::vector<Request> gather_requests(size_t b, const uint32_t* ids, const size_t
     return reqs;
 }
 
-void report(char* err, size_t len, const std::string& msg) {
-    if (!err || len == 0) return;
-    const size_t n = std::min(msg.size(), len - 1);
-    memcpy(err, msg.data(), n);
-    err[n] = 0;
-}
-
-template <typename F>
-int guarded(char* err, size_t len, F&& f) {
-    try {
-        f();
-        return 0;
-    } catch (const std::exception& ex) {
-        report(err, len, ex.what());
-    } catch (...) {
-        report(err, len, "julia-hip: unknown exception");
-    }
-    return -1;
-}
-
 // src/timing.rs:43-74: warm-up calls, then batches of back-to-back calls between two events,
 // one wait at the end; min and median per call.
 template <typename F>
@@ -755,10 +736,6 @@ void time_calls(F&& launch, int warmup, int batches, int per_batch, hipStream_t 
 }
 
 }  // namespace
-
-struct julia_hip_scratch {
-    Scratch s;
-};
 
 extern "C" {
 
@@ -842,8 +819,6 @@ static Gemm to_gemm(const julia_hip_gemm_args* g) {
     x.rope_rows = g->rope_rows, x.stats_out = g->stats_out;
     return x;
 }
-
-static Scratch scratch_of(const julia_hip_scratch* s) { return s ? s->s : Scratch{}; }
 
 int julia_hip_gemm(const julia_hip_gemm_args* g, julia_hip_gemm_config cfg,
                    const julia_hip_scratch* s, void* stream, char* err, size_t err_len) {

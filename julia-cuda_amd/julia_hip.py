@@ -60,6 +60,50 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+TYPES = {"f16": 0, "bf16": 1, "f32": 2}
+
+
+class AttentionBiasArgs(ctypes.Structure):
+    _fields_ = [
+        ("type", ctypes.c_int),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64),
+        ("kv_stride", ctypes.c_int64),
+        ("o", ctypes.c_void_p),
+        ("o_stride", ctypes.c_int64),
+        ("nq", ctypes.c_int),
+        ("nk", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("q_first", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("cap", ctypes.c_float),
+        ("table", ctypes.c_void_p),
+        ("bucket", ctypes.c_void_p),
+        ("buckets", ctypes.c_int),
+        ("reach", ctypes.c_int),
+        ("slopes", ctypes.c_void_p),
+        ("window", ctypes.c_int),
+        ("span", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+    ]
+
+
+class AttentionBiasGrads(ctypes.Structure):
+    _fields_ = [
+        ("dout", ctypes.c_void_p),
+        ("do_stride", ctypes.c_int64),
+        ("dq", ctypes.c_void_p),
+        ("dk", ctypes.c_void_p),
+        ("dv", ctypes.c_void_p),
+        ("dq_stride", ctypes.c_int64),
+        ("dkv_stride", ctypes.c_int64),
+        ("dtable", ctypes.c_void_p),
+    ]
+
+
 class GemmConfig(ctypes.Structure):
     _fields_ = [("bm", ctypes.c_int), ("splits", ctypes.c_int)]
 
@@ -95,6 +139,10 @@ EXPORTS = [
     "julia_hip_encode_batch",
     "julia_hip_encode_batch_phases", "julia_hip_checkpoint_config", "julia_hip_answer",
     "julia_hip_latency_summary",
+    "julia_hip_attention_bias", "julia_hip_attention_bias_backward",
+    "julia_hip_attention_bias_scratch", "julia_hip_attention_bias_check",
+    "julia_hip_layer_norm", "julia_hip_layer_norm_backward", "julia_hip_layer_norm_scratch",
+    "julia_hip_prep_relative_buckets", "julia_hip_prep_spans",
 ]
 
 _VP, _SZ, _I, _F, _CP = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float, ctypes.c_char_p
@@ -170,6 +218,19 @@ def lib():
                                      _CP, _SZ]),
         "julia_hip_encode_batch": (_I, [_VP, _SZ, _VP, _VP, _I, _VP, ctypes.POINTER(_F), _CP,
                                         _SZ]),
+        "julia_hip_attention_bias": (_I, [_VP, _VP, _VP, _CP, _SZ]),
+        "julia_hip_attention_bias_backward": (_I, [_VP, _VP, _VP, _VP, _CP, _SZ]),
+        "julia_hip_attention_bias_scratch": (_I, [_VP, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ),
+                                                  _CP, _SZ]),
+        "julia_hip_attention_bias_check": (_I, [_VP, _VP, _CP, _SZ]),
+        "julia_hip_layer_norm": (_I, [_I, _VP, ctypes.c_int64, _I, _I, _VP, _VP, _F, _VP,
+                                      ctypes.c_int64, _VP, _VP, _CP, _SZ]),
+        "julia_hip_layer_norm_backward": (_I, [_I, _VP, ctypes.c_int64, _VP, ctypes.c_int64, _I, _I,
+                                               _VP, _VP, _VP, ctypes.c_int64, _VP, _VP, _VP, _VP,
+                                               _CP, _SZ]),
+        "julia_hip_layer_norm_scratch": (_I, [_I, _I, ctypes.POINTER(_SZ), _CP, _SZ]),
+        "julia_hip_prep_relative_buckets": (_I, [_I, _I, _I, _I, _I32P, _CP, _SZ]),
+        "julia_hip_prep_spans": (_I, [_VP, _VP, _SZ, _VP, _CP, _SZ]),
         "julia_hip_encode_batch_phases": (_I, [_VP, _SZ, _VP, _VP, ctypes.POINTER(_F), _CP, _SZ]),
     }
     for name, (res, args) in sig.items():
@@ -517,7 +578,93 @@ def score(y, n, d, w, b, markers, k, logits, stream=0):
     _call(lib().julia_hip_score, y, n, d, w, b, markers, k, logits, stream or None)
 
 
+def attention_bias_args(type, q, k, v, o, nq, nk, heads, kv_heads=0, q_stride=0, kv_stride=0,
+                        o_stride=0, q_first=0, scale=0.125, cap=0.0, table=0, bucket=0, buckets=0,
+                        reach=0, slopes=0, window=0, span=0, lse=0):
+    """The arguments of attention_bias (device addresses); a program keeps them for its buffers.
+    type: "f16" or "bf16". kv_heads 0: heads. Strides 0: rows end to end."""
+    kv_heads = kv_heads or heads
+    return AttentionBiasArgs(TYPES[type], q or None, k or None, v or None, q_stride or 64 * heads,
+                             kv_stride or 64 * kv_heads, o or None, o_stride or 64 * heads, nq, nk,
+                             heads, kv_heads, q_first, scale, cap, table or None, bucket or None,
+                             buckets, reach, slopes or None, window, span or None, lse or None)
+
+
+def attention_bias_grads(args, dout, dq, dk, dv, do_stride=0, dq_stride=0, dkv_stride=0, dtable=0):
+    """The gradients that attention_bias_backward takes (dout) and writes, for a call's arguments.
+    Strides 0: rows end to end."""
+    d, kv = 64 * args.heads, 64 * args.kv_heads
+    return AttentionBiasGrads(dout or None, do_stride or d, dq or None, dk or None, dv or None,
+                              dq_stride or d, dkv_stride or kv, dtable or None)
+
+
+def attention_bias_scratch(args, backward=False):
+    """(ws_floats, counters) of the Scratch that the call takes."""
+    ws, counters = ctypes.c_size_t(), ctypes.c_size_t()
+    _call(lib().julia_hip_attention_bias_scratch, ctypes.byref(args), int(backward),
+          ctypes.byref(ws), ctypes.byref(counters))
+    return ws.value, counters.value
+
+
+def attention_bias(args, scratch=None, stream=0):
+    """Attention with capped scores, a bias by distance and spans of keys (julia_hip_attention_bias)."""
+    _call(lib().julia_hip_attention_bias, ctypes.byref(args), scratch.ptr if scratch else None,
+          stream or None)
+
+
+def attention_bias_backward(args, grads, scratch=None, stream=0):
+    """Its gradients, from the o and lse that the forward call left."""
+    _call(lib().julia_hip_attention_bias_backward, ctypes.byref(args), ctypes.byref(grads),
+          scratch.ptr if scratch else None, stream or None)
+
+
+def layer_norm(type, x, rows, d, gamma, beta, eps, y, x_stride=0, y_stride=0, stats=0, stream=0):
+    """Layer norm over rows of d values of `type` ("f16", "bf16", "f32"); strides 0: d."""
+    _call(lib().julia_hip_layer_norm, TYPES[type], x, x_stride or d, rows, d, gamma, beta or None, eps,
+          y, y_stride or d, stats or None, stream or None)
+
+
+def layer_norm_scratch(rows, d):
+    """(ws_floats, counters) of the Scratch that layer_norm_backward takes."""
+    ws = ctypes.c_size_t()
+    _call(lib().julia_hip_layer_norm_scratch, rows, d, ctypes.byref(ws))
+    return ws.value, 0
+
+
+def layer_norm_backward(type, x, dy, rows, d, gamma, stats, dx, dgamma, dbeta=0, x_stride=0,
+                        dy_stride=0, dx_stride=0, scratch=None, stream=0):
+    _call(lib().julia_hip_layer_norm_backward, TYPES[type], x, x_stride or d, dy, dy_stride or d, rows,
+          d, gamma, stats, dx, dx_stride or d, dgamma, dbeta or None, scratch.ptr if scratch else None,
+          stream or None)
+
+
 # ---------------------------------------------------------------- Part 3: host logic
+def attention_bias_check(args, grads=None):
+    """attention_bias's checks (with grads: its gradients') on the host; raises JuliaHipError."""
+    _call(lib().julia_hip_attention_bias_check, ctypes.byref(args),
+          ctypes.byref(grads) if grads else None)
+
+
+def relative_buckets(buckets, max_distance, both=True, reach=None):
+    """The bucket of each distance key - query from -reach (default: max_distance) to reach."""
+    reach = max_distance if reach is None else reach
+    out = np.empty(2 * max(reach, 0) + 1, np.int32)
+    _call(lib().julia_hip_prep_relative_buckets, buckets, max_distance, int(both), reach, out)
+    return out
+
+
+def spans(lens, prefix=None):
+    """Each row's keys [first, one past last) for documents of these lengths end to end: its whole
+    document, or (prefix: a number of rows a document) its prefix and the rows up to itself."""
+    n = np.ascontiguousarray(lens, np.uintp)
+    p = None if prefix is None else np.ascontiguousarray(prefix, np.uintp)
+    if p is not None and len(p) != len(n):
+        raise JuliaHipError(f"spans: {len(p)} prefixes for {len(n)} documents")
+    out = np.empty((int(n.sum()), 2), np.int32)
+    _call(lib().julia_hip_prep_spans, _np_ptr(n), _np_ptr(p), len(n), _np_ptr(out))
+    return out
+
+
 def fold_layernorm(w, gamma):
     w = np.ascontiguousarray(w, np.float32)
     out, k = w.shape

@@ -1,0 +1,579 @@
+"""The biased attention, layer norm and their gradients on the GPU, against their formulas in 64 bits
+(tests/relative.py), at the sizes, masks and values where they can go wrong."""
+
+import math
+
+import numpy as np
+import pytest
+
+import julia_hip as jh
+
+pytestmark = pytest.mark.gpu
+
+BUCKETS, REACH = 32, 128
+
+
+def say(*a):
+    print(*a, flush=True)
+
+
+@pytest.fixture(scope="module")
+def R(torch_cuda):
+    import relative
+
+    return relative
+
+
+def stream(torch):
+    return torch.cuda.current_stream().cuda_stream
+
+
+class Attention:
+    """A problem's tensors: a packed qkv (with `pad` columns and rows around it), its bias and spans."""
+
+    def __init__(self, torch, R, type, nq, nk=None, heads=2, kv=None, bias="none", cap=0.0, window=0, lens=None,
+                 prefix=None, span=None, seed=0, std=1.3, reach=REACH, pad=0, scale=0.125, dstd=0.05):
+        nk = nq if nk is None else nk
+        kv = kv or heads
+        g = torch.Generator().manual_seed(seed)
+        self.torch, self.R, self.type, self.nq, self.nk, self.heads, self.kv = torch, R, type, nq, nk, heads, kv
+        self.dt = R.DTYPE[type]
+        rnd = lambda *s: torch.randn(*s, generator=g)
+        width = (heads + 2 * kv) * 64 + pad
+        self.width = width
+        qkv = rnd(nk + 8, width)
+        qkv[:, : (heads + kv) * 64] *= std
+        self.qkv = qkv.to(self.dt).cuda()
+        self.first = nk - nq
+        self.kw = dict(scale=scale, cap=cap, window=window, q_first=self.first)
+        self.table = self.bucket = self.slopes = self.span = None
+        if bias == "table":
+            self.table = rnd(BUCKETS, heads).cuda()
+            self.bucket = torch.from_numpy(jh.relative_buckets(BUCKETS, max(reach, 9), reach=reach)).cuda()
+            self.kw.update(table=self.table, bucket=self.bucket, reach=reach)
+        elif bias == "slopes":
+            self.slopes = torch.exp2(-8.0 * torch.arange(1, heads + 1) / heads).cuda()
+            self.kw.update(slopes=self.slopes)
+        self.reach = reach
+        if lens is not None:
+            span = torch.from_numpy(jh.spans(lens, prefix))[-nq:]
+        if span is not None:
+            self.span = span.to(torch.int32).contiguous().cuda()
+            self.kw.update(span=self.span)
+        self.dout = (dstd * rnd(nq + 1, heads * 64)).to(self.dt).cuda()
+        self.fill()
+
+    def parts(self, t):
+        h, kv = self.heads, self.kv
+        return (t[self.first:self.nk, : h * 64].reshape(-1, h, 64), t[: self.nk, h * 64:(h + kv) * 64].reshape(-1, kv, 64),
+                t[: self.nk, (h + kv) * 64:(h + 2 * kv) * 64].reshape(-1, kv, 64))
+
+    def fill(self):
+        """Fresh outputs, filled with a value that no result has, one row longer than needed."""
+        t, d = self.torch, self.heads * 64
+        self.o = t.full((self.nq + 1, d), 777.0, dtype=self.dt, device="cuda")
+        self.lse = t.full((self.heads * self.nq + 1,), 777.0, device="cuda")
+        self.dqkv = t.full_like(self.qkv, 777.0)
+        self.dtable = None if self.table is None else t.full_like(self.table, 777.0)
+
+    def args(self, save=True):
+        p = lambda t: 0 if t is None else t.data_ptr()
+        e, h, kv = self.qkv.element_size(), self.heads, self.kv
+        base = self.qkv.data_ptr()
+        k = base + 64 * h * e
+        return jh.attention_bias_args(
+            self.type, base + self.first * self.width * e, k, k + 64 * kv * e, self.o.data_ptr(), self.nq, self.nk, h,
+            kv, q_stride=self.width, kv_stride=self.width, q_first=self.first, scale=self.kw["scale"],
+            cap=self.kw["cap"], table=p(self.table), bucket=p(self.bucket), buckets=BUCKETS, reach=self.reach,
+            slopes=p(self.slopes), window=self.kw["window"], span=p(self.span), lse=p(self.lse) if save else 0)
+
+    def grads(self, a):
+        e, h, kv = self.qkv.element_size(), self.heads, self.kv
+        base = self.dqkv.data_ptr()
+        k = base + 64 * h * e
+        return jh.attention_bias_grads(a, self.dout.data_ptr(), base + self.first * self.width * e, k, k + 64 * kv * e,
+                                       dq_stride=self.width, dkv_stride=self.width,
+                                       dtable=0 if self.dtable is None else self.dtable.data_ptr())
+
+    def forward(self, save=True):
+        a = self.args(save)
+        with_scratch(jh.attention_bias_scratch(a), lambda s: jh.attention_bias(a, scratch=s, stream=stream(self.torch)))
+        self.torch.cuda.synchronize()
+
+    def backward(self):
+        a = self.args()
+        with_scratch(jh.attention_bias_scratch(a, backward=True),
+                     lambda s: jh.attention_bias_backward(a, self.grads(a), scratch=s, stream=stream(self.torch)))
+        self.torch.cuda.synchronize()
+
+    def reference(self, back):
+        q, k, v = self.parts(self.qkv)
+        kw = dict(self.kw)
+        return self.R.attention(q, k, v, dout=self.dout[: self.nq].reshape(-1, self.heads, 64) if back else None, **kw)
+
+    def check(self, back=True):
+        """Runs the forward pass, with `back` the gradients too, and holds them to the formula."""
+        self.forward()
+        if back:
+            self.backward()
+        ref = self.reference(back)
+        bound = self.R.attention_bounds(ref, self.type, self.kw["cap"])
+        got = {"o": self.o[: self.nq].reshape(-1, self.heads, 64), "lse": self.lse[:-1].reshape(self.heads, self.nq)}
+        if back:
+            got["dq"], got["dk"], got["dv"] = self.parts(self.dqkv)
+            if self.dtable is not None:
+                got["dtable"] = self.dtable
+        off = {x: self.R.worst(y, ref[x], bound[x]) for x, y in got.items()}
+        say("   ", {x: round(y, 3) for x, y in off.items()})
+        assert max(off.values()) <= 1.0, off
+        # nothing past the rows, nor between them
+        assert bool((self.o[self.nq:] == 777.0).all()) and float(self.lse[-1]) == 777.0
+        if back:
+            used = self.torch.zeros_like(self.dqkv, dtype=self.torch.bool)
+            h, kv = self.heads * 64, self.kv * 64
+            used[self.first:self.nk, :h] = True
+            used[: self.nk, h:h + 2 * kv] = True
+            assert bool((self.dqkv[~used] == 777.0).all())
+        return ref, got
+
+
+def with_scratch(size, call):
+    s = jh.Scratch(*size)
+    try:
+        call(s)
+        jh.sync()
+    finally:
+        s.close()
+
+
+CASES = [
+    dict(type="f16", nq=1), dict(type="bf16", nq=2, bias="table"), dict(type="f16", nq=16, bias="slopes"),
+    dict(type="f16", nq=63, bias="table", heads=3), dict(type="f16", nq=64, bias="none", heads=1),
+    dict(type="bf16", nq=65, bias="slopes", heads=4, kv=2), dict(type="f16", nq=129, bias="table", heads=6, kv=2),
+    dict(type="f16", nq=293, bias="table", heads=12), dict(type="bf16", nq=293, bias="table", heads=12, kv=4, cap=50.0),
+    dict(type="f16", nq=200, bias="none", cap=5.0), dict(type="f16", nq=200, bias="slopes", cap=30.0, kv=1),
+    dict(type="f16", nq=321, bias="table", window=64), dict(type="bf16", nq=321, bias="none", window=1),
+    dict(type="f16", nq=448, bias="table", lens=[100, 1, 7, 64, 276]),
+    dict(type="bf16", nq=448, bias="table", lens=[100, 1, 7, 64, 276], prefix=[30, 0, 7, 1, 100], heads=6, kv=2),
+    dict(type="f16", nq=400, bias="slopes", lens=[400], prefix=[0], cap=20.0),
+    dict(type="f16", nq=700, bias="table", heads=12, lens=[300, 400], window=64),
+    dict(type="f16", nq=300, bias="table", reach=0), dict(type="f16", nq=300, bias="table", reach=5),
+    dict(type="f16", nq=600, bias="table", reach=512, heads=1), dict(type="f16", nq=150, pad=24, bias="table"),
+    dict(type="f16", nq=1500, heads=4, bias="table", lens=[1500], prefix=[500]),
+]
+
+
+def name(c):
+    return "-".join(f"{k}{v}" if k != "type" else v for k, v in c.items()).replace(" ", "")
+
+
+@pytest.mark.parametrize("case", CASES, ids=name)
+def test_attention_and_its_gradients(torch_cuda, R, case):
+    say("attention", case)
+    Attention(torch_cuda, R, seed=len(str(case)), **case).check()
+
+
+FEW = [dict(nq=1, nk=1), dict(nq=1, nk=5000, bias="slopes"), dict(nq=1, nk=4097, heads=12, kv=4, bias="table"),
+       dict(nq=3, nk=1000, heads=6, kv=2, cap=30.0, bias="table"), dict(nq=17, nk=2049, heads=2, window=64, bias="table"),
+       dict(nq=40, nk=900, heads=4, kv=1, bias="slopes"), dict(nq=70, nk=333, heads=3, bias="none")]
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("case", FEW, ids=name)
+def test_few_queries_over_many_keys(torch_cuda, R, case, type):
+    """The queries stand at the last rows; the gradients' kernels take them as well."""
+    say("few queries", case, type)
+    Attention(torch_cuda, R, type=type, seed=3, **case).check()
+
+
+@pytest.mark.parametrize("bias", ["none", "table", "slopes"])
+@pytest.mark.parametrize("cap", [0.0, 10.0])
+def test_spans_that_leave_rows_empty_and_are_out_of_range(torch_cuda, R, bias, cap):
+    torch = torch_cuda
+    n = 150
+    span = torch.tensor([[0, n]] * n)
+    span[3] = torch.tensor([40, 40])    # none
+    span[64:90] = torch.tensor([9, 2])  # none, the wrong way round
+    span[90] = torch.tensor([-2 ** 31, 2 ** 31 - 1])  # cut to the rows there are
+    span[91] = torch.tensor([n, 2 * n])
+    span[128:] = torch.tensor([5, 6])
+    say("odd spans", bias, cap)
+    A = Attention(torch, R, "f16", n, heads=3, bias=bias, cap=cap, span=span.long(), seed=5)
+    ref, got = A.check()
+    assert bool((got["o"][64:90] == 0).all()) and bool((got["lse"][:, 64:90] == -math.inf).all())
+    assert bool((got["dq"][64:90] == 0).all())
+    # every row empty
+    A = Attention(torch, R, "bf16", 70, heads=2, bias=bias, cap=cap, span=torch.zeros(70, 2).long(), seed=5)
+    ref, got = A.check()
+    assert all(bool((got[x] == 0).all()) for x in ("o", "dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_masked_infinities_and_nan_stay_where_they_are(torch_cuda, R, type):
+    """Rows 100.. of two documents in one tile hold NaN and infinities in k, v, q and dout: the first
+    document's results are those of the first document alone, bit for bit or within the bound."""
+    torch = torch_cuda
+    n, first = 160, 100
+    say("masked NaN", type)
+    A = Attention(torch, R, type, n, heads=4, kv=2, bias="table", lens=[first, n - first], seed=7)
+    A.qkv[first + 3, 64 * 4:] = math.nan
+    A.qkv[first + 5, 64 * 4:] = math.inf
+    A.qkv[first + 9, 64 * 7] = -math.inf
+    A.qkv[first + 20, :64] = math.nan
+    A.dout[first + 30] = math.nan
+    A.qkv[n:] = math.nan  # behind the last document
+    A.forward()
+    A.backward()
+    B = Attention(torch, R, type, first, heads=4, kv=2, bias="table", seed=7)
+    B.qkv[:first], B.dout[:first], B.table = A.qkv[:first], A.dout[:first], A.table
+    B.kw["table"] = B.table
+    ref = B.reference(True)
+    bound = R.attention_bounds(ref, type)
+    dq, dk, dv = A.parts(A.dqkv)
+    got = {"o": A.o[:first].reshape(-1, 4, 64), "lse": A.lse[:-1].reshape(4, n)[:, :first], "dq": dq[:first],
+           "dk": dk[:first], "dv": dv[:first]}
+    off = {x: R.worst(y, ref[x], bound[x]) for x, y in got.items()}
+    say("   ", off)
+    assert max(off.values()) <= 1.0, off
+    assert bool(torch.isnan(A.o[first:n]).any())
+    # a key that later queries alone see
+    A = Attention(torch, R, type, 130, heads=2, lens=[130], prefix=[0], seed=8)
+    A.qkv[70, 64 * 4:] = math.inf
+    A.forward()
+    ref = R.attention(*(t[:70] for t in A.parts(A.qkv)), span=A.span[:70])
+    assert R.worst(A.o[:70].reshape(-1, 2, 64), ref["o"], R.attention_bounds(ref, type)["o"]) <= 1.0
+    assert not bool(torch.isfinite(A.o[70:130, 64:]).all(1).any())
+
+
+def test_biases_of_the_lowest_value(torch_cuda, R):
+    """A bucket of the lowest f32 leaves its keys no weight; where every key has it, all have the same,
+    and -inf in every key is a row that sees none."""
+    torch = torch_cuda
+    low = torch.finfo(torch.float32).min
+    for value in (low, -math.inf):
+        say("bias", value)
+        A = Attention(torch, R, "f16", 140, heads=2, bias="table", seed=11)
+        A.table[3] = value
+        A.table[24:] = value
+        ref, got = A.check()
+        A = Attention(torch, R, "f16", 90, heads=2, bias="table", seed=12)
+        A.table[:] = value
+        A.forward()
+        o = A.o[:90].reshape(90, 2, 64).double().cpu()
+        if value == low:
+            mean = A.parts(A.qkv)[2].double().cpu().mean(0)
+            assert float((o - mean[None]).abs().max()) <= 2.0 ** -11 * 4
+            A.backward()
+            assert bool((A.dqkv[:90] == 0).all()) and bool((A.dtable == 0).all())
+        else:
+            assert bool((o == 0).all()) and bool((A.lse[:-1] == -math.inf).all())
+
+
+def test_small_and_large_gradients_in_f16(torch_cuda, R):
+    """Gradients of a loss's mean are small and those of a scaled loss large: dS is scaled by a power
+    of two before it is rounded, so both keep the type's precision (results that f16 itself cannot
+    hold apart)."""
+    torch = torch_cuda
+    for dstd in (2.0 ** -9, 1.0, 2.0 ** 10):
+        say("dout of", dstd)
+        A = Attention(torch, R, "f16", 260, heads=2, bias="table", dstd=dstd, seed=13)
+        A.check()
+    # a scale of 1 and wide scores (a few keys have all the weight)
+    Attention(torch, R, "f16", 260, heads=2, bias="table", scale=1.0, std=1.0, seed=14).check()
+
+
+def test_the_same_bits_at_every_call(torch_cuda, R):
+    torch = torch_cuda
+    A = Attention(torch, R, "f16", 900, heads=6, kv=2, bias="table", lens=[400, 500], seed=15)
+    A.forward()
+    A.backward()
+    want = [t.clone() for t in (A.o, A.lse, A.dqkv, A.dtable)]
+    for _ in range(3):
+        A.fill()
+        A.forward()
+        A.backward()
+        for x, y in zip((A.o, A.lse, A.dqkv, A.dtable), want):
+            assert torch.equal(x, y)
+    A.fill()
+    A.forward(save=False)
+    assert torch.equal(A.o, want[0]) and bool((A.lse == 777.0).all())
+
+
+def test_gradients_against_differences(torch_cuda, R):
+    """The gradients are those of the forward kernel: the loss sum(o . w) along a direction of the
+    table, by central differences. With steps of 2^-3 in the table the difference is off by the third
+    derivative, about step^2 / 6 of the loss's size, and by the rounding of the weights and of o to f16
+    in either of the two, 2 2^-11 of it over the step."""
+    torch = torch_cuda
+    A = Attention(torch, R, "f16", 200, heads=2, bias="table", cap=30.0, seed=16, dstd=1.0)
+    A.forward()
+    A.backward()
+    w = A.dout[:200].double()
+    loss = lambda: float((A.o[:200].double() * w).sum())
+    size = float((A.o[:200].double().abs() * w.abs()).sum())
+    direction = torch.randn(A.table.shape, generator=torch.Generator().manual_seed(1)).cuda()
+    table, step, by = A.table.clone(), 2.0 ** -3, []
+    for sign in (1, -1):
+        A.table.copy_(table + sign * step * direction)
+        A.forward()
+        by.append(loss())
+    A.table.copy_(table)
+    want, got = (by[0] - by[1]) / (2 * step), float((A.dtable.double() * direction.double()).sum())
+    say("differences:", want, got, size)
+    assert abs(want - got) <= size * (step ** 2 / 6 * 8 + 2 * 2.0 ** -11 / step)
+
+
+@pytest.mark.parametrize("back", [False, True])
+def test_captured_and_on_another_stream(torch_cuda, R, back):
+    """Two graphs that share a scratch, replayed one after the other with eager calls between them."""
+    torch = torch_cuda
+    P = [Attention(torch, R, "f16", 260, heads=4, kv=2, bias="table", seed=17),
+         Attention(torch, R, "bf16", 4, nk=3000, heads=6, kv=2, bias="slopes", seed=18)]
+    if back:
+        P[1] = Attention(torch, R, "bf16", 131, heads=6, kv=2, cap=20.0, bias="table", seed=18)
+    sizes = [jh.attention_bias_scratch(A.args(), backward=b) for A in P for b in (False, True)]
+    scratch = jh.Scratch(max(s[0] for s in sizes), max(s[1] for s in sizes))
+    side = torch.cuda.Stream()
+
+    def call(A, st):
+        a = A.args()
+        if back:
+            jh.attention_bias_backward(a, A.grads(a), scratch=scratch, stream=st)
+        else:
+            jh.attention_bias(a, scratch=scratch, stream=st)
+
+    outs = lambda A: [t for t in ((A.dqkv, A.dtable) if back else (A.o, A.lse)) if t is not None]
+    want, graphs = [], []
+    for A in P:
+        A.forward()
+        with torch.cuda.stream(side):
+            call(A, side.cuda_stream)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in outs(A)])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            call(A, side.cuda_stream)
+        graphs.append(g)
+    for rep in range(3):
+        for A, g, w in zip(P, graphs, want):
+            for t in outs(A):
+                t.fill_(777.0)
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(outs(A), w)), f"replay {rep}"
+            call(A, stream(torch))
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(outs(A), w)), f"after replay {rep}"
+    scratch.close()
+
+
+def test_rows_far_into_a_long_cache(torch_cuda, R):
+    """Keys whose addresses pass 32 bits: rows 2^20 elements apart."""
+    torch = torch_cuda
+    nk, wide = 2300, 1 << 20  # 4.5 GB
+    A = Attention(torch, R, "f16", 2, nk=nk, heads=2, bias="slopes", seed=19)
+    big = torch.zeros(nk, wide, dtype=torch.float16, device="cuda")
+    big[:, : A.width] = A.qkv[:nk]
+    A.forward()
+    want = A.o.clone()
+    a = A.args()
+    a.k, a.v, a.kv_stride = big.data_ptr() + 64 * 2 * 2, big.data_ptr() + 64 * 4 * 2, wide
+    A.o.fill_(777.0)
+    with_scratch(jh.attention_bias_scratch(a), lambda s: jh.attention_bias(a, scratch=s, stream=stream(torch)))
+    assert torch.equal(A.o, want)
+    # the gradients over keys that far apart
+    A = Attention(torch, R, "f16", nk, heads=2, bias="slopes", seed=20, window=64)
+    big[:, : A.width] = A.qkv[:nk]
+    A.forward()
+    A.backward()
+    want = A.dqkv.clone()
+    a = A.args()
+    a.k, a.v, a.kv_stride = big.data_ptr() + 64 * 2 * 2, big.data_ptr() + 64 * 4 * 2, wide
+    A.dqkv.fill_(777.0)
+    with_scratch(jh.attention_bias_scratch(a, backward=True),
+                 lambda s: jh.attention_bias_backward(a, A.grads(a), scratch=s, stream=stream(torch)))
+    assert torch.equal(A.dqkv, want)
+
+
+def test_a_scratch_that_is_too_small_is_refused(torch_cuda, R):
+    torch = torch_cuda
+    A = Attention(torch, R, "f16", 1, nk=4000, heads=2, seed=21)
+    a = A.args()
+    with pytest.raises(jh.JuliaHipError, match="the scratch has"):
+        jh.attention_bias(a, stream=stream(torch))
+    with pytest.raises(jh.JuliaHipError, match="the scratch has"):
+        jh.attention_bias_backward(a, A.grads(a), stream=stream(torch))
+    with pytest.raises(jh.JuliaHipError, match="the scratch has"):
+        jh.layer_norm_backward("f16", A.qkv.data_ptr(), A.qkv.data_ptr(), 4, 64, A.lse.data_ptr(), A.lse.data_ptr(),
+                               A.dqkv.data_ptr(), A.lse.data_ptr())
+    torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------- layer norm
+def norm_problem(torch, R, type, rows, d, shift, seed, pad=0, offset=0):
+    g = torch.Generator().manual_seed(seed)
+    dt = R.DTYPE[type]
+    make = lambda s: (s * torch.randn(rows + 1, d + pad + offset, generator=g) + 0.5).to(dt).cuda()[:, offset:offset + d]
+    P = {"x": make(2.0), "dy": make(0.1), "gamma": (1 + 0.2 * torch.randn(d, generator=g)).cuda()}
+    P["beta"] = (0.1 * torch.randn(d, generator=g)).cuda() if shift else None
+    P["y"] = torch.full((rows + 1, d + pad + offset), 777.0, dtype=dt, device="cuda")[:, offset:offset + d]
+    P["dx"] = torch.full_like(P["y"], 777.0)
+    P["stats"] = torch.full((rows + 1, 2), 777.0, device="cuda")
+    P["dgamma"], P["dbeta"] = (torch.full((d + 1,), 777.0, device="cuda") for _ in range(2))
+    return P
+
+
+NORMS = [(1, 1), (3, 2), (5, 7), (1, 64), (293, 768), (100, 1000), (33, 1001), (70, 384), (9, 1536), (5, 2048),
+         (6, 2049), (3, 4096), (2, 8192), (7, 5003), (3000, 96)]
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,d", NORMS)
+@pytest.mark.parametrize("layout", ["end to end", "apart", "odd"])
+def test_layer_norm_and_its_gradients(torch_cuda, R, type, rows, d, layout):
+    """A row's mean and deviation are f32 sums over d values (2^-24 a term at most, in a tree: some
+    2^-20), y is rounded once; dx's terms are f32 and dx is rounded once."""
+    torch = torch_cuda
+    pad, offset = {"end to end": (0, 0), "apart": (8, 0), "odd": (2, 1)}[layout]
+    shift = (rows + d) % 2 == 0
+    say("norm", type, rows, d, layout)
+    P = norm_problem(torch, R, type, rows, d, shift, rows + d, pad, offset)
+    ptr = lambda t: 0 if t is None else t.data_ptr()
+    st = dict(x_stride=P["x"].stride(0), stream=stream(torch))
+    jh.layer_norm(type, ptr(P["x"]), rows, d, ptr(P["gamma"]), ptr(P["beta"]), 1e-5, ptr(P["y"]),
+                  y_stride=P["y"].stride(0), stats=ptr(P["stats"]), **st)
+    torch.cuda.synchronize()
+    ref = R.norm(P["x"][:rows], P["gamma"], P["beta"], 1e-5, P["dy"][:rows])
+    u, f = R.U[type], 2.0 ** -19
+    tiny = 2.0 ** -24 if type == "f16" else 1e-30
+    size = P["x"][:rows].double().cpu().abs().mean(1, keepdim=True) * ref["rstd"][:, None]
+    mag = (ref["xh"].abs() + size) * P["gamma"].double().cpu().abs()
+    off = {"y": R.worst(P["y"][:rows], ref["y"], u * ref["y"].abs() + f * (mag + ref["y"].abs()) + tiny),
+           "mean": R.worst(P["stats"][:rows, 0], ref["mean"], f * P["x"][:rows].double().cpu().abs().mean(1) + 1e-30),
+           "rstd": R.worst(P["stats"][:rows, 1], ref["rstd"], f * ref["rstd"] * (1 + size[:, 0]))}
+    with_scratch(jh.layer_norm_scratch(rows, d), lambda s: jh.layer_norm_backward(
+        type, ptr(P["x"]), ptr(P["dy"]), rows, d, ptr(P["gamma"]), ptr(P["stats"]), ptr(P["dx"]), ptr(P["dgamma"]),
+        ptr(P["dbeta"]) if shift else 0, dy_stride=P["dy"].stride(0), dx_stride=P["dx"].stride(0), scratch=s, **st))
+    off["dx"] = R.worst(P["dx"][:rows], ref["dx"], u * ref["dx"].abs() + 4 * f * (1 + size) * ref["dx_sum"] + tiny)
+    terms = (P["dy"][:rows].double().cpu().abs() * size).sum(0)
+    off["dgamma"] = R.worst(P["dgamma"][:d], ref["dgamma"], 2 * f * (ref["dgamma_sum"] + terms) + 1e-30)
+    if shift:
+        off["dbeta"] = R.worst(P["dbeta"][:d], ref["dbeta"], f * ref["dbeta_sum"] + 1e-30)
+    say("   ", {x: round(y, 3) for x, y in off.items()})
+    assert max(off.values()) <= 1.0, off
+    assert bool((P["y"][rows:] == 777.0).all()) and bool((P["stats"][rows:] == 777.0).all())
+    assert bool((P["dx"][rows:] == 777.0).all()) and float(P["dgamma"][d]) == 777.0
+    assert shift or bool((P["dbeta"] == 777.0).all())
+    base = P["y"]._base
+    if base is not None and (pad or offset):
+        assert bool((base[:, :offset] == 777.0).all()) and bool((base[:, offset + d:] == 777.0).all())
+
+
+def test_layer_norm_of_no_rows_in_place_and_captured(torch_cuda, R):
+    torch = torch_cuda
+    ptr = lambda t: t.data_ptr()
+    P = norm_problem(torch, R, "f16", 500, 768, True, 3)
+    scratch = jh.Scratch(*jh.layer_norm_scratch(500, 768))
+
+    def back(dx, rows=500, st=None):
+        jh.layer_norm_backward("f16", ptr(P["x"]), ptr(P["dy"]), rows, 768, ptr(P["gamma"]), ptr(P["stats"]), ptr(dx),
+                               ptr(P["dgamma"]), ptr(P["dbeta"]), scratch=scratch, stream=stream(torch) if st is None else st)
+
+    def forward(y, rows=500):
+        jh.layer_norm("f16", ptr(P["x"]), rows, 768, ptr(P["gamma"]), ptr(P["beta"]), 1e-5, ptr(y), stats=ptr(P["stats"]),
+                      stream=stream(torch))
+
+    # no rows: nothing is written but gradients of zero
+    forward(P["y"], 0)
+    back(P["dx"], 0)
+    torch.cuda.synchronize()
+    assert bool((P["y"] == 777.0).all()) and bool((P["dx"] == 777.0).all())
+    assert bool((P["dgamma"][:768] == 0).all()) and bool((P["dbeta"][:768] == 0).all())
+    forward(P["y"])
+    back(P["dx"])
+    torch.cuda.synchronize()
+    want = [P[x].clone() for x in ("dx", "dgamma", "dbeta")]
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        back(P["dx"], st=side.cuda_stream)
+    for _ in range(3):
+        for x in ("dx", "dgamma", "dbeta"):
+            P[x].fill_(777.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(P["dx"][:500], want[0][:500]) and torch.equal(P["dgamma"][:768], want[1][:768])
+        assert torch.equal(P["dbeta"][:768], want[2][:768])
+        back(P["dx"])
+        torch.cuda.synchronize()
+    # in place: y over x, dx over dy
+    y, dy = P["y"].clone(), P["dy"].clone()
+    back(P["dy"])
+    torch.cuda.synchronize()
+    assert torch.equal(P["dy"][:500], want[0][:500])
+    P["dy"].copy_(dy)
+    forward(P["x"])
+    torch.cuda.synchronize()
+    assert torch.equal(P["x"][:500], y[:500])
+    scratch.close()
+
+
+# ---------------------------------------------------------------- together
+def test_a_layer_forward_and_back(torch_cuda, R):
+    """Norm, attention with a learned bias over two documents, and the residual, as a pre-norm encoder
+    layer chains them, and its gradients (by x, the projections, gamma and the table) against the same
+    layer's in 64 bits by torch's own differentiation. The products between are torch's, in f32 from the
+    f16 values, so what the operators round is what may differ: each of five roundings (norm, qkv, o, the
+    two gradients of them) by 2^-11 of its value, and no gradient's norm by more than a few of them."""
+    torch = torch_cuda
+    n, heads, d = 230, 4, 256
+    g = torch.Generator().manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, generator=g)
+    x = rnd(n, d).half().cuda()
+    wqkv, wo = (rnd(3 * d, d) / 16).cuda(), (rnd(d, d) / 16).cuda()
+    gamma, beta = (1 + 0.1 * rnd(d)).cuda(), (0.1 * rnd(d)).cuda()
+    table, dout = rnd(BUCKETS, heads).cuda(), (0.1 * rnd(n, d)).cuda()
+    bucket = torch.from_numpy(jh.relative_buckets(BUCKETS, REACH)).cuda()
+    span = torch.from_numpy(jh.spans([100, 130])).cuda()
+    st, ptr = stream(torch), lambda t: t.data_ptr()
+    empty = lambda *s, dtype=torch.float16: torch.empty(*s, dtype=dtype, device="cuda")
+
+    h, stats = empty(n, d), empty(n, 2, dtype=torch.float32)
+    jh.layer_norm("f16", ptr(x), n, d, ptr(gamma), ptr(beta), 1e-5, ptr(h), stats=ptr(stats), stream=st)
+    qkv = (h.float() @ wqkv.T).half()
+    o, lse = empty(n, d), empty(heads, n, dtype=torch.float32)
+    a = jh.attention_bias_args("f16", ptr(qkv), ptr(qkv) + 2 * d, ptr(qkv) + 4 * d, ptr(o), n, n, heads, q_stride=3 * d,
+                               kv_stride=3 * d, table=ptr(table), bucket=ptr(bucket), buckets=BUCKETS, reach=REACH,
+                               span=ptr(span), lse=ptr(lse))
+    sizes = [jh.attention_bias_scratch(a), jh.attention_bias_scratch(a, backward=True), jh.layer_norm_scratch(n, d)]
+    scratch = jh.Scratch(max(s[0] for s in sizes), max(s[1] for s in sizes))
+    jh.attention_bias(a, scratch=scratch, stream=st)
+    y = x.float() + o.float() @ wo.T
+    do = (dout @ wo).half()
+    dqkv, dtable = empty(n, 3 * d), torch.empty_like(table)
+    gr = jh.attention_bias_grads(a, ptr(do), ptr(dqkv), ptr(dqkv) + 2 * d, ptr(dqkv) + 4 * d, dq_stride=3 * d,
+                                 dkv_stride=3 * d, dtable=ptr(dtable))
+    jh.attention_bias_backward(a, gr, scratch=scratch, stream=st)
+    dh, dx = (dqkv.float() @ wqkv).half(), empty(n, d)
+    dgamma, dbeta = empty(d, dtype=torch.float32), empty(d, dtype=torch.float32)
+    jh.layer_norm_backward("f16", ptr(x), ptr(dh), n, d, ptr(gamma), ptr(stats), ptr(dx), ptr(dgamma), ptr(dbeta),
+                           scratch=scratch, stream=st)
+    got = {"y": y, "x": dx.float() + dout, "wqkv": dqkv.float().T @ h.float(), "wo": dout.T @ o.float(), "gamma": dgamma,
+           "beta": dbeta, "table": dtable}
+    torch.cuda.synchronize()
+    scratch.close()
+
+    leaf = {k: v.double().cpu().requires_grad_() for k, v in
+            dict(x=x, wqkv=wqkv, wo=wo, gamma=gamma, beta=beta, table=table).items()}
+    hh = torch.nn.functional.layer_norm(leaf["x"], (d,), leaf["gamma"], leaf["beta"], 1e-5)
+    q, k, v = (hh @ leaf["wqkv"].T).reshape(n, 3, heads, 64).permute(1, 2, 0, 3)
+    t = torch.arange(n)[None] - torch.arange(n)[:, None]
+    s = q @ k.transpose(1, 2) / 8 + leaf["table"][bucket.cpu().long()[t.clamp(-REACH, REACH) + REACH]].permute(2, 0, 1)
+    doc = torch.arange(n) >= 100
+    s = s.masked_fill(doc[:, None] != doc[None], -math.inf)
+    yy = leaf["x"] + (torch.softmax(s, 2) @ v).transpose(0, 1).reshape(n, d) @ leaf["wo"].T
+    yy.backward(dout.double().cpu())
+    for key, value in got.items():
+        want = yy.detach() if key == "y" else leaf[key].grad
+        rel = float((value.double().cpu() - want).norm() / want.norm())
+        say("   ", key, rel)
+        assert rel <= 8 * 2.0 ** -11, key
