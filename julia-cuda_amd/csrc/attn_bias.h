@@ -48,7 +48,7 @@ struct AttnBiasGrads {
 constexpr int BIAS_PAD = 80;
 constexpr int BIAS_MAX_REACH = 512;
 // LDS for the tables of the query heads that share a key head, in floats.
-constexpr int BIAS_MAX_TABLE = 8000;
+constexpr int BIAS_MAX_TABLE = 6000;
 inline int bias_row(int reach) { return 2 * (reach + BIAS_PAD) + 1; }
 
 struct ScratchSize {

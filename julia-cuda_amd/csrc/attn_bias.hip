@@ -133,33 +133,10 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
         const int kb = k0 + 64 * (c0 + kg + KS * b);
         const bool act = has(b) && !(kb + 64 <= wlo || kb >= whi);
         const char* st = ring + ST * 16384;
-        floatx4 sc[4];
+        floatx4 sc[4], base[4];  // (base: the scores' initial values; with a cap, what is added after it)
         half4 vlo[2][4], vhi[2][4];
         if (act) {
-            // the scores' initial values (with a cap, what is added after it)
-            floatx4 base[4];
-            if (BIAS == BIAS_TABLE) {
-                if (kb - wql >= p.reach || kb + 63 - wq0 <= -p.reach) {
-                    const float b0 = kb > wq0 ? right : left;
-#pragma unroll
-                    for (int t = 0; t < 4; t++) base[t] = floatx4{b0, b0, b0, b0};
-                } else {
-                    const float* at = tab + (kb + 4 * g - qpos);
-#pragma unroll
-                    for (int t = 0; t < 4; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) base[t][e] = at[16 * t + e];
-                }
-            } else if (BIAS == BIAS_SLOPES) {
-                const float x = (float)(kb + 4 * g - qpos);
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) base[t][e] = fmaf(-slope, fabsf(x + (float)(16 * t + e)), p.off);
-            } else {
-#pragma unroll
-                for (int t = 0; t < 4; t++) base[t] = CAP ? floatx4{p.off, p.off, p.off, p.off} : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
+            block_bias<BIAS>(p, tab, left, right, slope, kb, g, qpos, wq0, wql, base);
             half8 kf[4][2];
 #pragma unroll
             for (int t = 0; t < 4; t++)
@@ -180,20 +157,12 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
                     vlo[hf][dt] = lds_read_tr16(st + voff[dt] + 4096 * hf);
                     vhi[hf][dt] = lds_read_tr16(st + voff[dt] + 4096 * hf + 2048);
                 }
-            if (CAP) {
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float r = __builtin_amdgcn_rcpf(fast_exp2(sc[t][e] * p.pre) + 1.0f);
-                        sc[t][e] = fmaf(-2.0f * p.off, r, base[t][e]);
-                    }
-            }
         }
         __builtin_amdgcn_sched_barrier(0);
         if (has(b + 1)) stage(kg + KS * (b + 1), (ST + 1) % 2);
         __builtin_amdgcn_sched_barrier(0);
         if (!act) return;
+        if (CAP) cap_scores<4, false>(p, sc, base, 1.0f);
         if (!(kb >= flo && kb + 64 <= fhi)) {
             const int at = kb + 4 * g - kr.lo;
 #pragma unroll
@@ -330,9 +299,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
 #pragma unroll
         for (int e = 0; e < 4; e++) bad |= !(fabsf(o[dt][e]) < INFINITY);
     }
-    uint64_t again = __builtin_amdgcn_ballot_w64(bad && row < rows);
-    again = (again | again >> 32) & 0xffffffffull;
-    again = (again | again >> 16) & 0xffffull;
+    uint64_t again = rows_where(bad && row < rows);
     const bool redo = (again >> r16) & 1;
     if (row < rows && !redo) {
         f16* op = p.o + (int64_t)qi * p.o_stride + h * 64 + 4 * g;
@@ -378,6 +345,7 @@ void attn_bias_check(const AttnBias& a, const AttnBiasGrads* g) {
     if (a.q_first < 0 || a.q_first >= (1 << 30)) fail("q_first must be from 0 to 2^30");
     if (!(a.scale >= 1e-6f && a.scale <= 1e6f)) fail("the scale must be from 1e-6 to 1e6");
     if (!(a.cap == 0.0f || (a.cap >= 1e-3f && a.cap <= 1e6f))) fail("the cap must be 0 or from 1e-3 to 1e6");
+    if (a.cap > 0.0f && a.scale > 1e3f * a.cap) fail("the scale must be up to 1000 caps");
     if (a.window < 0 || a.window >= (1 << 30)) fail("the window must be from 0 to 2^30");
     if (a.table && a.slopes) fail("a bias table or slopes, not both");
     if (a.table) {
@@ -422,9 +390,15 @@ BiasParams bias_params(const AttnBias& a) {
     p.q_stride = a.q_stride, p.kv_stride = a.kv_stride, p.o_stride = a.o_stride;
     p.nq = a.nq, p.nk = a.nk, p.heads = a.heads, p.kv_heads = a.kv_heads, p.each = a.heads / a.kv_heads;
     p.q_first = a.q_first, p.scale = a.scale;
-    if (a.cap > 0.0f)
+    if (a.cap > 0.0f) {
         p.mul = 1.0f, p.unit = (float)log2e, p.off = (float)(a.cap * log2e), p.pre = (float)(2.0 * log2e * a.scale / a.cap);
-    else
+        // tanh(x) / x over 0 <= x^2 <= 1/4 by a polynomial of x^2 with the least relative error
+        // (a weighted least squares fit over Chebyshev points, reweighted until it is level: 1.3e-8)
+        const double c[5] = {0.9999999868719406, -0.3333306939409053, 0.13324779312866444, -0.05298607478007015, 0.01713500531796541};
+        const double x = (double)a.scale / a.cap;  // of q . k
+        for (int i = 0; i < 5; i++) p.poly[i] = (float)(c[i] * a.cap * log2e * pow(x, 2 * i + 1));
+        p.small = (float)(0.5 / x), p.per_off = (float)(1.0 / (a.cap * log2e));
+    } else
         p.mul = (float)(a.scale * log2e), p.unit = (float)(1.0 / a.scale), p.off = 0.0f, p.pre = 0.0f;
     p.table = a.table, p.bucket = a.bucket, p.buckets = a.buckets, p.reach = a.reach, p.row = a.table ? bias_row(a.reach) : 0;
     p.slopes = a.slopes, p.window = a.window, p.span = a.span, p.lse = a.lse;

@@ -10,8 +10,11 @@ namespace jh {
 // What the kernels take: the attention in the units they work in. Scores run in the exp2 domain:
 // without a cap the MFMA accumulates q . k + (bias / scale), and a weight is exp2 of that times
 // `mul` = scale log2(e) less the row's log-sum; with one, a score is
-//   cap log2(e) tanh(x) + bias log2(e) = (off + bias unit) - 2 off / (exp2(q . k pre) + 1)
-// with x = scale q . k / cap, pre = 2 log2(e) scale / cap, off = cap log2(e) and unit = log2(e) (`mul` is 1).
+//   cap log2(e) tanh(x) + bias log2(e) = off - 2 off / (exp2(q . k pre) + 1) + bias unit
+// with x = scale q . k / cap, pre = 2 log2(e) scale / cap, off = cap log2(e) and unit = log2(e) (`mul` is
+// 1). Where |x| <= 1/2 the tanh is x times a polynomial of x^2 instead (poly, in units of q . k and with off
+// taken in; |q . k| <= small): exact to 2^-24 of itself, where the other form is to 2^-23 of 1, which `off`
+// makes some 2^-17 of a score.
 struct BiasParams {
     const f16 *q, *k, *v;
     int64_t q_stride, kv_stride;
@@ -19,6 +22,7 @@ struct BiasParams {
     int64_t o_stride;
     int nq, nk, heads, kv_heads, each, q_first;
     float scale, mul, unit, off, pre;
+    float poly[5], small, per_off;  // (per_off: 1 / off)
     const float* table;
     const int32_t* bucket;
     int buckets, reach, row;  // row: floats of a head's padded distances in LDS
@@ -96,11 +100,11 @@ __device__ __forceinline__ KeyRange key_range(const BiasParams& p, int i) {
     return hi > lo ? KeyRange{lo, hi} : KeyRange{0, 0};
 }
 
-// A bias in the scores' units, plus the cap's offset. A finite one stays finite: where every key
+// A bias in the scores' units. A finite one stays finite: where every key
 // of a row has the lowest bias of the type, their weights are equal, as in the formula.
 __device__ __forceinline__ float bias_value(const BiasParams& p, float b) {
     const float v = b * p.unit;
-    return (fabsf(b) <= 3.4028234e38f ? fminf(fmaxf(v, -3.4028234e38f), 3.4028234e38f) : v) + p.off;
+    return (fabsf(b) <= 3.4028234e38f ? fminf(fmaxf(v, -3.4028234e38f), 3.4028234e38f) : v);
 }
 
 // The padded distances of `n` heads from `head` on into LDS: tab[x row + reach + BIAS_PAD + t] is
@@ -125,14 +129,49 @@ __device__ __forceinline__ float dot64(const f16* a, const f16* b) {
     return s;
 }
 
+// N x 4 capped scores in place from q . k, base in them; slope: the tanh's slope times `by`, into base.
+// Whether every one of the wave's is small is asked first: those of a model usually are, and the
+// polynomial takes 7 operations where the other takes 11 (an exponential and a reciprocal at four each).
+template <int N, bool SLOPE>
+__device__ __forceinline__ void cap_scores(const BiasParams& p, floatx4 (&sc)[N], floatx4 (&base)[N], float by) {
+    float most = 0.0f;
+#pragma unroll
+    for (int t = 0; t < N; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) most = fmaxf(most, fabsf(sc[t][e]));
+    if (__builtin_amdgcn_ballot_w64(!(most <= p.small)) == 0) {  // (NaN: the other form keeps it)
+#pragma unroll
+        for (int t = 0; t < N; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float z = sc[t][e] * sc[t][e];
+                const float v = sc[t][e] * fmaf(z, fmaf(z, fmaf(z, fmaf(z, p.poly[4], p.poly[3]), p.poly[2]), p.poly[1]), p.poly[0]);
+                sc[t][e] = v + base[t][e];
+                if (SLOPE) {
+                    const float y = v * p.per_off;
+                    base[t][e] = by * fmaf(-y, y, 1.0f);
+                }
+            }
+    } else {
+#pragma unroll
+        for (int t = 0; t < N; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float r = __builtin_amdgcn_rcpf(fast_exp2(sc[t][e] * p.pre) + 1.0f);
+                sc[t][e] = fmaf(-2.0f * p.off, r, base[t][e] + p.off);
+                if (SLOPE) base[t][e] = (4.0f * by) * fmaf(-r, r, r);
+            }
+    }
+}
+
 // A score's weight in the exp2 domain (before the row's log-sum is taken off) from q . k, the
-// tanh's slope in `slope` (1 without a cap). base: the bias in the scores' units plus the offset.
+// tanh's slope in `slope` (1 without a cap). base: the bias in the scores' units.
 template <bool CAP>
 __device__ __forceinline__ float score_of(const BiasParams& p, float qk, float base, float& slope) {
     if (CAP) {
         const float r = __builtin_amdgcn_rcpf(fast_exp2(qk * p.pre) + 1.0f);
         slope = 4.0f * fmaf(-r, r, r);
-        return fmaf(-2.0f * p.off, r, base);
+        return fmaf(-2.0f * p.off, r, base + p.off);
     }
     slope = 1.0f;
     return (qk + base) * p.mul;
@@ -142,8 +181,44 @@ __device__ __forceinline__ float score_of(const BiasParams& p, float qk, float b
 template <int BIAS>
 __device__ __forceinline__ float bias_at(const BiasParams& p, const float* tab, float slope, int t) {
     if (BIAS == BIAS_TABLE) return tab[min(max(t, -p.reach), p.reach) + p.reach + BIAS_PAD];
-    if (BIAS == BIAS_SLOPES) return fmaf(-slope, fabsf((float)t), p.off);
-    return p.off;
+    if (BIAS == BIAS_SLOPES) return -slope * fabsf((float)t);
+    return 0.0f;
+}
+
+// The biases of a 64-key block from kb on for a lane's query (S^T: keys kb + 16 t + 4 g + e): tab, the
+// lane's distance 0; left, right: the table's ends; wq0, wql: the wave's first and last query.
+template <int BIAS>
+__device__ __forceinline__ void block_bias(const BiasParams& p, const float* tab, float left, float right, float slope,
+                                           int kb, int g, int qpos, int wq0, int wql, floatx4 (&base)[4]) {
+    if (BIAS == BIAS_TABLE) {
+        if (kb - wql >= p.reach || kb + 63 - wq0 <= -p.reach) {
+            const float b0 = kb > wq0 ? right : left;
+#pragma unroll
+            for (int t = 0; t < 4; t++) base[t] = floatx4{b0, b0, b0, b0};
+        } else {
+            const float* at = tab + (kb + 4 * g - qpos);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) base[t][e] = at[16 * t + e];
+        }
+    } else if (BIAS == BIAS_SLOPES) {
+        const float x = (float)(kb + 4 * g - qpos);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) base[t][e] = -slope * fabsf(x + (float)(16 * t + e));
+    } else {
+#pragma unroll
+        for (int t = 0; t < 4; t++) base[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+}
+
+// Which of a wave's 16 rows (one a lane % 16) have a lane where `bad` holds.
+__device__ __forceinline__ uint64_t rows_where(bool bad) {
+    uint64_t b = __builtin_amdgcn_ballot_w64(bad);
+    b = (b | b >> 32) & 0xffffffffull;
+    return (b | b >> 16) & 0xffffull;
 }
 
 }  // namespace jh

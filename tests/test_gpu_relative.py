@@ -160,6 +160,8 @@ CASES = [
     dict(type="f16", nq=300, bias="table", reach=0), dict(type="f16", nq=300, bias="table", reach=5),
     dict(type="f16", nq=600, bias="table", reach=512, heads=1), dict(type="f16", nq=150, pad=24, bias="table"),
     dict(type="f16", nq=1500, heads=4, bias="table", lens=[1500], prefix=[500]),
+    dict(type="f16", nq=1400, heads=12, bias="table", lens=[300, 64, 500, 536]),
+    dict(type="bf16", nq=1100, heads=16, bias="slopes", cap=30.0, lens=[1100], prefix=[100]),
 ]
 
 

@@ -70,7 +70,7 @@ def grads(a, **kw):
 REFUSED = [(dict(nq=-1), "queries"), (dict(nk=1 << 30), "keys"), (dict(heads=0, kv_heads=1), "heads"),
            (dict(heads=5), "heads"), (dict(heads=257, kv_heads=257), "heads"), (dict(q_first=-1), "q_first"),
            (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=math.nan), "scale"),
-           (dict(scale=math.inf), "scale"), (dict(cap=-1.0), "cap"), (dict(cap=math.nan), "cap"),
+           (dict(scale=math.inf), "scale"), (dict(cap=-1.0), "cap"), (dict(cap=0.01, scale=100.0), "caps"), (dict(cap=math.nan), "cap"),
            (dict(window=-1), "window"), (dict(table=4, bucket=4, buckets=2, slopes=4), "not both"),
            (dict(table=4, buckets=2), "buckets"), (dict(table=4, bucket=4, buckets=0), "buckets"),
            (dict(table=4, bucket=4, buckets=2, reach=513), "reach"), (dict(table=4, bucket=4, buckets=2, reach=-1), "reach"),
@@ -117,8 +117,10 @@ def test_scratch_sizes():
     assert jh.attention_bias_scratch(args(nq=20000, nk=20000)) == (0, 0)
     floats, counters = jh.attention_bias_scratch(args(nq=1, nk=8192))
     assert counters == 2 and floats > 0
-    floats, _ = jh.attention_bias_scratch(args(nq=1000, nk=1000), backward=True)
-    assert floats >= 2 * 4 * 1000
+    floats, counters = jh.attention_bias_scratch(args(nq=1000, nk=1000), backward=True)
+    assert floats >= 2 * 4 * 1000 and counters == 0
+    a = args(nq=1000, nk=1000, table=4, bucket=4, buckets=2)
+    assert jh.attention_bias_scratch(a, backward=True)[1] == 4
     assert jh.layer_norm_scratch(0, 8)[0] >= 0 and jh.layer_norm_scratch(1000, 768)[0] > 0
 
 
