@@ -81,11 +81,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
     const f16* const qp = p.q + (int64_t)qi * p.q_stride + h * 64;
     const half8 qf[2] = {*(const half8*)(qp + 8 * g), *(const half8*)(qp + 32 + 8 * g)};
     const float slope = BIAS == BIAS_SLOPES ? p.slopes[h] * p.unit : 0.0f;
-    if (BIAS == BIAS_TABLE) load_bias(p, kvh * p.each, p.each, tab0, 64 * NW * KS);
     const float* const tab = tab0 + (BIAS == BIAS_TABLE ? hh * p.row + p.reach + BIAS_PAD : 0);  // distance 0
-    __syncthreads();
-    const float left = BIAS == BIAS_TABLE ? tab[-p.reach] : 0.0f, right = BIAS == BIAS_TABLE ? tab[p.reach] : 0.0f;
-
     const int blocks = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0;
     const int c0 = (int)((int64_t)chunk * blocks / p.chunks), nblk = (int)((int64_t)(chunk + 1) * blocks / p.chunks) - c0;
 
@@ -124,6 +120,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
 #pragma unroll
     for (int t = 0; t < 4; t++) o[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
+    float left = 0.0f, right = 0.0f;  // a table's ends
     const int nsteps = (nblk + KS - 1) / KS;
     auto has = [&](int b) { return kg + KS * b < nblk; };
     auto step = [&](int b, auto st_) {
@@ -222,7 +219,13 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
             }
         }
     };
+    // (the first copy goes out ahead of the table's two dependent loads)
     if (has(0)) stage(kg, 0);
+    if (BIAS == BIAS_TABLE) {
+        load_bias(p, kvh * p.each, p.each, tab0, 64 * NW * KS);
+        __syncthreads();
+        left = tab[-p.reach], right = tab[p.reach];
+    }
     for (int b = 0; b < nsteps; b += 2) {
         step(b, std::integral_constant<int, 0>{});
         if (b + 1 < nsteps) step(b + 1, std::integral_constant<int, 1>{});

@@ -5,9 +5,9 @@
 // Two launches, each over the scores again (seven products in place of five), so that no block adds to
 // another's results and the gradients are the same bits at every call:
 // - dq_kernel: 16 NW queries of a head over their keys: dQ, the rows' constants for the other (-lse,
-//   -D, their keys) and the sums of dS by distance.
+//   -D, their keys) and the block's sums of dS by bucket.
 // - dkv_kernel: 16 NG NW keys of a key head over the queries that see them: dK and dV; further blocks
-//   sum the distances' shares over the first launch's blocks, and into buckets.
+//   sum the buckets' shares over the first launch's blocks.
 //
 // - Both keep the scores where the next product wants them: a lane's column is its query (dQ) or its
 //   key (dK, dV), and the transposed operand comes from LDS by the transposing read.
@@ -21,7 +21,7 @@
 // - The bias's gradient in 32 bits, before dS is rounded: a 64-key block past `reach` on one side adds
 //   to one sum; else the 16 queries of a wave are summed along the diagonals with lane shifts (a
 //   lane's four keys of a 16-key tile against its neighbours' queries) and added to the wave's own
-//   row of distances in LDS.
+//   row of distances in LDS, which the block sums by bucket at its end.
 // - A row whose sums are not finite is computed again key by key over the pairs that are not masked: a
 //   masked infinity or NaN times a weight of 0 is NaN in the tile's products.
 #include <algorithm>
@@ -41,14 +41,12 @@ struct BiasBack {
     float* dtable;
     // The workspace: per head and (padded) row -lse log2(e) (-inf: a row without keys) and -D, per row
     // its keys (first, number), per 16 rows the keys (least first, most past last, most first, least
-    // past last) and a head's largest |dO|^2, per (head, block) the distances' sums, and the buckets'
-    // over `slices` of the blocks.
+    // past last) and a head's largest |dO|^2, per (head, block) the buckets' sums.
     float *nl, *dn;
     int2* range;
     int4* bounds;
-    float *max_do, *part, *sums;
-    uint32_t* counters;
-    int nqp, tiles, slices, dkv_blocks;  // tiles: a head's blocks of the first launch
+    float *max_do, *part;
+    int nqp, tiles, dkv_blocks;  // tiles: a head's blocks of the first launch
 };
 
 constexpr int DQ_STAGE = 16384;           // K and V of 64 keys
@@ -76,6 +74,29 @@ __device__ __forceinline__ void grad_pair(const BiasBack& b, const float* tab, f
     da = w * (dp + dn) * cap;
 }
 
+// out[x stride] = the sum of term(x, i) over i < n, for x < m, by a block: THREADS / (m rounded up to a
+// power of two) threads share an x, each taking every so-manyth i, and join in order. sm: THREADS floats.
+template <int THREADS, typename F>
+__device__ __forceinline__ void sum_groups(int m, int n, float* sm, float* out, int stride, F&& term) {
+    int wide = 1;
+    while (wide < m && wide < THREADS) wide *= 2;
+    const int parts = THREADS / wide, y = threadIdx.x / wide;
+    for (int x0 = 0; x0 < m; x0 += wide) {
+        const int x = x0 + threadIdx.x % wide;
+        float a = 0.0f;
+        if (x < m)
+#pragma unroll 8
+            for (int i = y; i < n; i += parts) a += term(x, i);
+        sm[threadIdx.x] = a;
+        __syncthreads();
+        if (y == 0 && x < m) {
+            for (int z = 1; z < parts; z++) a += sm[z * wide + threadIdx.x];
+            out[(size_t)x * stride] = a;
+        }
+        __syncthreads();
+    }
+}
+
 // ---- dQ of 16 NW queries of a head --------------------------------------------------------------
 template <bool BF, int BIAS, bool CAP, int NW, int KS>
 __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) {
@@ -89,8 +110,11 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     const int j4 = r16 >> 2, q4 = r16 & 3;
     const int dists = 2 * p.reach + 1;
     char* const ring = lds + kg * 2 * DQ_STAGE;
+    float* const ring0 = (float*)lds;
     float* const tab0 = (float*)(lds + KS * 2 * DQ_STAGE);
-    float* const hist = tab0 + p.row + wk * dists;
+    int* const bucket = (int*)(tab0 + p.row);
+    float* const hist0 = tab0 + p.row + dists;
+    float* const hist = hist0 + wk * dists;
 
     // The keys of the block's rows (lane l: row q0 + l), then the lane's own row.
     KeyRange tr{0, 0};
@@ -128,7 +152,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     auto has = [&](int s) { return kg + KS * s < nblk; };
     if (has(0)) stage(kg, 0);
     if (BIAS == BIAS_TABLE) {
-        load_bias(p, h, 1, tab0, 64 * NW * KS);
+        load_bias(p, h, 1, tab0, 64 * NW * KS, bucket);
         for (int i = l; i < dists; i += 64) hist[i] = 0.0f;
     }
 
@@ -162,9 +186,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
             b.dn[(size_t)h * b.nqp + row] = dn;
             if (h == 0) b.range[row] = make_int2(kr.lo, kr.hi - kr.lo);
         }
-        float m = sq;
-#pragma unroll
-        for (int s = 1; s < 16; s <<= 1) m = fmaxf(m, __shfl_xor(m, s));
+        const float m = row_max(sq);
         if (l == 0) {
             b.max_do[(size_t)h * (b.nqp / 16) + q0 / 16 + w] = m;
             if (h == 0) b.bounds[q0 / 16 + w] = make_int4(wlo, whi, flo, fhi);
@@ -311,14 +333,16 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     }
     __syncthreads();
     if (BIAS == BIAS_TABLE) {
-        float* to = b.part + ((size_t)h * b.tiles + tile) * dists;
-        const float* from = tab0 + p.row;
         for (int i = tid; i < dists; i += 64 * NW * KS) {
-            float s = from[i];
+            float s = hist0[i];
 #pragma unroll
-            for (int x = 1; x < NW * KS; x++) s += from[x * dists + i];
-            to[i] = s;
+            for (int x = 1; x < NW * KS; x++) s += hist0[x * dists + i];
+            hist0[i] = s;
         }
+        __syncthreads();
+        sum_groups<64 * NW * KS>(p.buckets, dists, ring0, b.part + ((size_t)h * b.tiles + tile) * p.buckets, 1,
+                                 [&](int x, int i) { return bucket[i] == x ? hist0[i] : 0.0f; });
+        __syncthreads();  // (the ring is free again)
     }
     if (KS > 1) {
         if (kg > 0) {
@@ -368,56 +392,17 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     }
 }
 
-// ---- the buckets' sums ------------------------------------------------------------------------
-// Slice s of head h's blocks: their sums by distance, then by bucket; the head's last slice to arrive
-// adds them up in order.
-template <int THREADS>
-__device__ __forceinline__ void table_sums(const BiasBack& b, int task, float* sm, uint32_t* s_last) {
-    const int dists = 2 * b.p.reach + 1, h = task / b.slices, s = task % b.slices, tid = threadIdx.x;
-    const int t0 = (int)((int64_t)s * b.tiles / b.slices), t1 = (int)((int64_t)(s + 1) * b.tiles / b.slices);
-    int* const bucket = (int*)(sm + dists);
-    for (int i = tid; i < dists; i += THREADS) {
-        const float* from = b.part + ((size_t)h * b.tiles + t0) * dists + i;
-        float a = 0.0f;
-#pragma unroll 8
-        for (int t = t0; t < t1; t++, from += dists) a += *from;
-        sm[i] = a;
-        bucket[i] = min(max(b.p.bucket[i], 0), b.p.buckets - 1);
-    }
-    __syncthreads();
-    float* const mine = b.sums + ((size_t)h * b.slices + s) * b.p.buckets;
-    for (int x = tid; x < b.p.buckets; x += THREADS) {
-        float a = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < dists; i++) a += bucket[i] == x ? sm[i] : 0.0f;
-        xstore32(mine + x, a);
-    }
-    release_wait();
-    __syncthreads();
-    if (tid == 0) {
-        const uint32_t last = atomic_add_agent(b.counters + h, 1u) == (uint32_t)(b.slices - 1);
-        if (last) atomic_store_agent(b.counters + h, 0u);
-        *s_last = last;
-    }
-    __syncthreads();
-    if (*s_last == 0) return;
-    for (int x = tid; x < b.p.buckets; x += THREADS) {
-        const float* from = b.sums + (size_t)h * b.slices * b.p.buckets + x;
-        float a = 0.0f;
-        for (int z = 0; z < b.slices; z++) a += xload32(from + (size_t)z * b.p.buckets);
-        b.dtable[(size_t)x * b.p.heads + h] = a;
-    }
-}
-
 // ---- dK and dV of 16 NG NW keys -----------------------------------------------------------------
 template <bool BF, int BIAS, bool CAP, int NG, int NW, int KS>
 __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b) {
     const BiasParams& p = b.p;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ uint32_t s_last;
     constexpr int WK = 16 * NG, KB = WK * NW, LOADS = 16 / NW;
     if (BIAS == BIAS_TABLE && (int)blockIdx.x >= b.dkv_blocks) {
-        table_sums<64 * NW * KS>(b, blockIdx.x - b.dkv_blocks, (float*)lds, &s_last);
+        const int h = blockIdx.x - b.dkv_blocks;
+        const float* from = b.part + (size_t)h * b.tiles * p.buckets;
+        sum_groups<64 * NW * KS>(p.buckets, b.tiles, (float*)lds, b.dtable + h, p.heads,
+                                 [&](int x, int i) { return from[(size_t)i * p.buckets + x]; });
         return;
     }
     const int tiles = (p.nk + KB - 1) / KB;
@@ -467,9 +452,8 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
                     m = fmaxf(m, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])));
                 }
         }
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) m = fmaxf(m, __shfl_xor(m, s));
-        sigma = grad_scale(m);
+        m = row_max(m);
+        sigma = grad_scale(max_xor32(max_xor16(m)));
     }
 #pragma unroll
     for (int x = 0; x < NG; x++)
@@ -773,15 +757,14 @@ GradPlan grad_plan(const AttnBias& a, int cus) {
 
 // The workspace's parts, in floats, each on 256 bytes.
 struct Layout {
-    size_t nl, dn, range, bounds, max_do, part, sums, all;
-    int nqp, tiles, slices;
+    size_t nl, dn, range, bounds, max_do, part, all;
+    int nqp, tiles;
 };
 
 Layout layout(const AttnBias& a, const GradPlan& plan) {
     Layout y{};
     y.nqp = (a.nq + 63) / 64 * 64;
     y.tiles = y.nqp / (16 * plan.dq_nw);
-    y.slices = std::max(1, std::min(16, y.tiles / 16));
     auto take = [&](size_t floats) {
         const size_t at = y.all;
         y.all += (floats + 63) / 64 * 64;
@@ -790,8 +773,7 @@ Layout layout(const AttnBias& a, const GradPlan& plan) {
     y.nl = take((size_t)a.heads * y.nqp), y.dn = take((size_t)a.heads * y.nqp);
     y.range = take(2 * (size_t)y.nqp), y.bounds = take(4 * (size_t)(y.nqp / 16));
     y.max_do = take((size_t)a.heads * (y.nqp / 16));
-    y.part = take(a.table ? (size_t)a.heads * y.tiles * (2 * a.reach + 1) : 0);
-    y.sums = take(a.table ? (size_t)a.heads * y.slices * a.buckets : 0);
+    y.part = take(a.table ? (size_t)a.heads * y.tiles * a.buckets : 0);
     return y;
 }
 
@@ -806,9 +788,9 @@ template <bool BF, int BIAS, bool CAP, int NW, int KS>
 void launch_dq(const BiasBack& b, hipStream_t st) {
     constexpr int ring = KS * 2 * DQ_STAGE, waves = NW * KS;
     static const bool ok = lds_limit(attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>,
-                                     ring + 4 * (bias_row(BIAS_MAX_REACH) + waves * (2 * BIAS_MAX_REACH + 1)));
+                                     ring + 4 * (bias_row(BIAS_MAX_REACH) + (waves + 1) * (2 * BIAS_MAX_REACH + 1)));
     (void)ok;
-    const size_t lds = ring + (BIAS == BIAS_TABLE ? 4 * (b.p.row + waves * (2 * (size_t)b.p.reach + 1)) : 0);
+    const size_t lds = ring + (BIAS == BIAS_TABLE ? 4 * (b.p.row + (waves + 1) * (2 * (size_t)b.p.reach + 1)) : 0);
     hipLaunchKernelGGL((attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>), dim3(b.tiles * b.p.heads), dim3(64 * waves), lds, st, b);
 }
 
@@ -818,7 +800,7 @@ void launch_dkv(BiasBack b, hipStream_t st) {
     static const bool ok = lds_limit(attn_bias_dkv_kernel<BF, BIAS, CAP, NG, NW, KS>, ring + 4 * BIAS_MAX_TABLE);
     (void)ok;
     b.dkv_blocks = (b.p.nk + 16 * NG * NW - 1) / (16 * NG * NW) * b.p.kv_heads;
-    const int blocks = b.dkv_blocks + (BIAS == BIAS_TABLE ? b.slices * b.p.heads : 0);
+    const int blocks = b.dkv_blocks + (BIAS == BIAS_TABLE ? b.p.heads : 0);
     const size_t lds = ring + (BIAS == BIAS_TABLE ? 4 * (size_t)b.p.each * b.p.row : 0);
     if (blocks) hipLaunchKernelGGL((attn_bias_dkv_kernel<BF, BIAS, CAP, NG, NW, KS>), dim3(blocks), dim3(64 * NW * KS), lds, st, b);
 }
@@ -841,24 +823,22 @@ void launch_type(const BiasBack& b, const GradPlan& plan, int bias, bool cap, hi
 }  // namespace
 
 ScratchSize attn_bias_backward_scratch(const AttnBias& a, int cus) {
-    return {layout(a, grad_plan(a, cus)).all, a.table ? (size_t)a.heads : 0};
+    return {layout(a, grad_plan(a, cus)).all, 0};
 }
 
 void attn_bias_backward_launch(const AttnBias& a, const AttnBiasGrads& g, const Scratch& s, hipStream_t st) {
     attn_bias_check(a, &g);
     const GradPlan plan = grad_plan(a, device_cus());
     const Layout y = layout(a, plan);
-    if (y.all > s.ws_floats || (a.table && (size_t)a.heads > s.n_counters))
-        fail("the scratch has " + std::to_string(s.ws_floats) + " floats and " + std::to_string(s.n_counters) + " counters, not " +
-             std::to_string(y.all) + " and " + std::to_string(a.table ? a.heads : 0));
+    if (y.all > s.ws_floats) fail("the scratch has " + std::to_string(s.ws_floats) + " floats, not " + std::to_string(y.all));
     BiasBack b{};
     b.p = bias_params(a);
-    b.nqp = y.nqp, b.tiles = y.tiles, b.slices = y.slices;
+    b.nqp = y.nqp, b.tiles = y.tiles;
     b.dout = (const f16*)g.dout, b.do_stride = g.do_stride;
     b.dq = (f16*)g.dq, b.dk = (f16*)g.dk, b.dv = (f16*)g.dv;
     b.dq_stride = g.dq_stride, b.dkv_stride = g.dkv_stride, b.dtable = g.dtable;
     b.nl = s.ws + y.nl, b.dn = s.ws + y.dn, b.range = (int2*)(s.ws + y.range), b.bounds = (int4*)(s.ws + y.bounds);
-    b.max_do = s.ws + y.max_do, b.part = s.ws + y.part, b.sums = s.ws + y.sums, b.counters = s.counters;
+    b.max_do = s.ws + y.max_do, b.part = s.ws + y.part;
     const int bias = a.table ? BIAS_TABLE : a.slopes ? BIAS_SLOPES : BIAS_NONE;
     a.bf16 ? launch_type<true>(b, plan, bias, a.cap > 0.0f, st) : launch_type<false>(b, plan, bias, a.cap > 0.0f, st);
     const hipError_t e = hipGetLastError();

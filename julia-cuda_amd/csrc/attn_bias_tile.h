@@ -72,15 +72,26 @@ __device__ __forceinline__ float widen(f16 v) {
     return (float)v;
 }
 
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) v = min(v, __shfl_xor(v, s));
-    return __builtin_amdgcn_readfirstlane(v);
+// The least and the most of a wave's values, to all lanes, without LDS (a shuffle's round trip is some
+// 100 clocks, and a block takes six such results before its first product): within 16 lanes by DPP,
+// as group_sum, then the lane swaps.
+template <int CTRL>
+__device__ __forceinline__ int dpp_int(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
 }
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) v = max(v, __shfl_xor(v, s));
-    return __builtin_amdgcn_readfirstlane(v);
+__device__ __forceinline__ int wave_min(int v) {
+    v = min(v, dpp_int<0xB1>(v)), v = min(v, dpp_int<0x4E>(v));
+    v = min(v, dpp_int<0x141>(v)), v = min(v, dpp_int<0x140>(v));
+    const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = min((int)a[0], (int)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return __builtin_amdgcn_readfirstlane(min((int)b[0], (int)b[1]));
+}
+__device__ __forceinline__ int wave_max(int v) { return ~wave_min(~v); }
+// The most of 16 lanes' values, none negative, to each of them.
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp_move<0xB1>(v)), v = fmaxf(v, dpp_move<0x4E>(v));
+    return v = fmaxf(v, dpp_move<0x141>(v)), fmaxf(v, dpp_move<0x140>(v));
 }
 
 // The keys that query i sees, [lo, hi) within [0, nk); none: lo = hi = 0.
@@ -108,11 +119,12 @@ __device__ __forceinline__ float bias_value(const BiasParams& p, float b) {
 }
 
 // The padded distances of `n` heads from `head` on into LDS: tab[x row + reach + BIAS_PAD + t] is
-// the bias of head + x at distance t (key - query).
-__device__ __forceinline__ void load_bias(const BiasParams& p, int head, int n, float* tab, int threads) {
+// the bias of head + x at distance t (key - query). bucket (nullable): the buckets of [-reach, reach].
+__device__ __forceinline__ void load_bias(const BiasParams& p, int head, int n, float* tab, int threads, int* bucket = nullptr) {
     for (int i = threadIdx.x; i < p.row; i += threads) {
         const int t = min(max(i - BIAS_PAD, 0), 2 * p.reach);
         const int b = min(max(p.bucket[t], 0), p.buckets - 1);
+        if (bucket) bucket[t] = b;  // (the padding writes its end's again)
         for (int x = 0; x < n; x++) tab[x * p.row + i] = bias_value(p, p.table[(size_t)b * p.heads + head + x]);
     }
 }

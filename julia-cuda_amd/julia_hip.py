@@ -12,6 +12,7 @@ The library must be built (`make -C julia-cuda_amd`); there is no fallback.
 import ctypes
 import os
 import sys
+import threading
 
 import numpy as np
 
@@ -245,8 +246,14 @@ def _err():
     return ctypes.create_string_buffer(ERR_LEN)
 
 
+_THREAD = threading.local()  # a thread's error buffer (making one costs a microsecond a call)
+
+
 def _call(fn, *args):
-    e = _err()
+    try:
+        e = _THREAD.err
+    except AttributeError:
+        e = _THREAD.err = _err()
     rc = fn(*args, e, ERR_LEN)
     if rc != 0:
         raise JuliaHipError(e.value.decode(errors="replace"))
