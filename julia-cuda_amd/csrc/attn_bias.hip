@@ -20,7 +20,7 @@
 
 namespace jh {
 
-constexpr int BIAS_RING = 2 * 16384;  // two stages of 64 keys: K, then V
+constexpr int BIAS_STAGE = 16384;  // 64 keys: K, then V
 
 // The row's output again, key by key over the keys it sees: a masked key's V may hold infinities
 // or NaN, which a weight of 0 in the tile's product would turn into NaN for rows that do not see it.
@@ -46,44 +46,44 @@ __device__ float bias_row_again(const BiasParams& p, const f16* qp, int kvh, int
 
 template <bool BF, int BIAS, bool CAP, int NW, int KS>
 __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    // The two stages are arrays of their own, so that the compiler can tell a copy into one from the reads
+    // of the other: in one array every LDS read waits for every copy in flight.
+    __shared__ __attribute__((aligned(16))) char stage0[KS * BIAS_STAGE], stage1[KS * BIAS_STAGE];
+    extern __shared__ __attribute__((aligned(16))) float tab0[];
     __shared__ uint32_t s_last;
     constexpr int QB = 16 * NW, LOADS = 16 / NW;
-    const int rows = p.nq * p.each, tiles = (rows + QB - 1) / QB;
-    const int task = xcd_task(blockIdx.x, tiles * p.kv_heads * p.chunks);
-    const int chunk = task % p.chunks, tile = task / p.chunks;
-    const int kvh = tile / tiles, r0 = (tile % tiles) * QB;
+    const int rows = p.nq * p.each;
+    const Quotient ct = divide(xcd_task(blockIdx.x, gridDim.x), p.by_chunks), ht = divide(ct.q, p.by_tiles);
+    const int chunk = ct.r, tile = ct.q, kvh = ht.q, r0 = ht.r * QB;
     const int tid = threadIdx.x, l = tid & 63, r16 = l & 15, g = l >> 4;
     const int wk = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int w = wk % NW, kg = wk / NW;
-    char* const ring = lds + kg * BIAS_RING;
-    float* const tab0 = (float*)(lds + KS * BIAS_RING);
     const int j4 = r16 >> 2, q4 = r16 & 3;
 
     // The keys of the block's rows (lane l: row r0 + l), of this wave's 16 and of the lane's own.
     const int mine = r0 + l;
+    const bool real = l < QB && mine < rows;
     KeyRange tr{0, 0};
-    if (l < QB && mine < rows) tr = key_range(p, mine / p.each);
-    const bool some = tr.hi > tr.lo;
-    const int k0 = wave_min(some ? tr.lo : 0x7fffffff);
-    const int k1 = wave_max(tr.hi);
-    const bool in_wave = (l >> 4) == w && mine < rows;
-    const int wlo = wave_min(in_wave && some ? tr.lo : 0x7fffffff), whi = wave_max(in_wave ? tr.hi : 0);
-    const int flo = wave_max(in_wave ? tr.lo : 0), fhi = wave_min(in_wave ? tr.hi : 0x7fffffff);
-
+    if (real) tr = key_range(p, divide(mine, p.by_each).q);
     const int row = r0 + 16 * w + r16;
-    const int rc = min(row, rows - 1);
-    const int qi = rc / p.each, hh = rc - qi * p.each, h = kvh * p.each + hh;
+    const Quotient qh = divide(min(row, rows - 1), p.by_each);
+    const int qi = qh.q, hh = qh.r, h = kvh * p.each + hh;
     const int qpos = p.q_first + qi;
-    const KeyRange kr = row < rows ? key_range(p, qi) : KeyRange{0, 0};
-    const uint32_t kspan = (uint32_t)(kr.hi - kr.lo);
-    const int wq0 = __builtin_amdgcn_readfirstlane(qpos), wql = p.q_first + min(r0 + 16 * w + 15, rows - 1) / p.each;
     const f16* const qp = p.q + (int64_t)qi * p.q_stride + h * 64;
     const half8 qf[2] = {*(const half8*)(qp + 8 * g), *(const half8*)(qp + 32 + 8 * g)};
+    const KeyBounds kb_ = key_bounds(tr, real, w);
+    const int k0 = kb_.k0, k1 = kb_.k1, wlo = kb_.lo, whi = kb_.hi, flo = kb_.flo, fhi = kb_.fhi;
+    const KeyRange kr = {__shfl(tr.lo, 16 * w + r16), __shfl(tr.hi, 16 * w + r16)};
+    const uint32_t kspan = (uint32_t)(kr.hi - kr.lo);
+    const int wq0 = __builtin_amdgcn_readfirstlane(qpos), wql = __builtin_amdgcn_readlane(qpos, 15);
     const float slope = BIAS == BIAS_SLOPES ? p.slopes[h] * p.unit : 0.0f;
     const float* const tab = tab0 + (BIAS == BIAS_TABLE ? hh * p.row + p.reach + BIAS_PAD : 0);  // distance 0
     const int blocks = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0;
-    const int c0 = (int)((int64_t)chunk * blocks / p.chunks), nblk = (int)((int64_t)(chunk + 1) * blocks / p.chunks) - c0;
+    int c0 = 0, nblk = blocks;
+    if (p.chunks > 1) {  // (blocks are below 2^24, chunks up to 256)
+        c0 = (uint32_t)(chunk * blocks) / (uint32_t)p.chunks;
+        nblk = (uint32_t)((chunk + 1) * blocks) / (uint32_t)p.chunks - c0;
+    }
 
     uint32_t doff[LOADS];
 #pragma unroll
@@ -91,8 +91,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
         const int c = ((w + NW * qq) & 7) * 64 + l, r = c >> 3, ch = (c & 7) ^ (r & 7);
         doff[qq] = (uint32_t)(r * (int)p.kv_stride * 2 + ch * 16);
     }
-    auto stage = [&](int b, int st) {
-        char* dst = ring + st * 16384;
+    auto stage = [&](int b, char* dst) {
         const int kb = k0 + 64 * (c0 + b);
         const uint32_t bytes = (uint32_t)((min(k1 - kb, 64) - 1) * (int)p.kv_stride * 2 + 128);
         const auto rk = buffer_rsrc(p.k + (int64_t)kb * p.kv_stride + kvh * 64, bytes);
@@ -125,14 +124,15 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
     auto has = [&](int b) { return kg + KS * b < nblk; };
     auto step = [&](int b, auto st_) {
         constexpr int ST = decltype(st_)::value;
-        wait_vmcnt<0>();
-        __builtin_amdgcn_s_barrier();
+        stage_barrier();
         const int kb = k0 + 64 * (c0 + kg + KS * b);
         const bool act = has(b) && !(kb + 64 <= wlo || kb >= whi);
-        const char* st = ring + ST * 16384;
+        const char* st = (ST ? stage1 : stage0) + kg * BIAS_STAGE;
+        if (has(b + 1)) stage(kg + KS * (b + 1), (ST ? stage0 : stage1) + kg * BIAS_STAGE);
+        if (!act) return;
         floatx4 sc[4], base[4];  // (base: the scores' initial values; with a cap, what is added after it)
         half4 vlo[2][4], vhi[2][4];
-        if (act) {
+        {
             block_bias<BIAS>(p, tab, left, right, slope, kb, g, qpos, wq0, wql, base);
             half8 kf[4][2];
 #pragma unroll
@@ -155,10 +155,6 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
                     vhi[hf][dt] = lds_read_tr16(st + voff[dt] + 4096 * hf + 2048);
                 }
         }
-        __builtin_amdgcn_sched_barrier(0);
-        if (has(b + 1)) stage(kg + KS * (b + 1), (ST + 1) % 2);
-        __builtin_amdgcn_sched_barrier(0);
-        if (!act) return;
         if (CAP) cap_scores<4, false>(p, sc, base, 1.0f);
         if (!(kb >= flo && kb + 64 <= fhi)) {
             const int at = kb + 4 * g - kr.lo;
@@ -220,7 +216,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
         }
     };
     // (the first copy goes out ahead of the table's two dependent loads)
-    if (has(0)) stage(kg, 0);
+    if (has(0)) stage(kg, stage0 + kg * BIAS_STAGE);
     if (BIAS == BIAS_TABLE) {
         load_bias(p, kvh * p.each, p.each, tab0, 64 * NW * KS);
         __syncthreads();
@@ -244,7 +240,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
         if (KS == 1) return;
         __syncthreads();
         if (kg > 0) {
-            float* mg = (float*)lds + ((kg - 1) * NW + w) * 18 * 64;
+            float* mg = (float*)stage0 + ((kg - 1) * NW + w) * 18 * 64;
             mg[16 * 64 + l] = mx;
             mg[17 * 64 + l] = sum;
 #pragma unroll
@@ -253,7 +249,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
         __syncthreads();
         if (kg == 0)
             for (int k = 1; k < KS; k++) {
-                const float* mg = (const float*)lds + ((k - 1) * NW + w) * 18 * 64;
+                const float* mg = (const float*)stage0 + ((k - 1) * NW + w) * 18 * 64;
                 floatx4 ok[4];
 #pragma unroll
                 for (int f = 0; f < 16; f++) ok[f >> 2][f & 3] = mg[f * 64 + l];
@@ -315,7 +311,8 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
     while (again) {
         const int x = __builtin_ctzll(again);
         again &= again - 1;
-        const int r = r0 + 16 * w + x, i = r / p.each, y = r - i * p.each, hx = kvh * p.each + y;
+        const Quotient r = divide(r0 + 16 * w + x, p.by_each);
+        const int i = r.q, y = r.r, hx = kvh * p.each + y;
         const float s1 = BIAS == BIAS_SLOPES ? p.slopes[hx] * p.unit : 0.0f;
         const float v = bias_row_again<BF, BIAS, CAP>(p, p.q + (int64_t)i * p.q_stride + hx * 64, kvh, p.q_first + i,
                                                       key_range(p, i), tab0 + y * p.row, s1, __shfl(mx, x), __shfl(total, x));
@@ -392,6 +389,7 @@ BiasParams bias_params(const AttnBias& a) {
     p.q = (const f16*)a.q, p.k = (const f16*)a.k, p.v = (const f16*)a.v, p.o = (f16*)a.o;
     p.q_stride = a.q_stride, p.kv_stride = a.kv_stride, p.o_stride = a.o_stride;
     p.nq = a.nq, p.nk = a.nk, p.heads = a.heads, p.kv_heads = a.kv_heads, p.each = a.heads / a.kv_heads;
+    p.by_each = Div(p.each);
     p.q_first = a.q_first, p.scale = a.scale;
     if (a.cap > 0.0f) {
         p.mul = 1.0f, p.unit = (float)log2e, p.off = (float)(a.cap * log2e), p.pre = (float)(2.0 * log2e * a.scale / a.cap);
@@ -430,9 +428,9 @@ template <bool BF, int BIAS, bool CAP, int NW, int KS>
 void launch_tile(const BiasParams& p, long tiles, hipStream_t st) {
     static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_bias_kernel<BF, BIAS, CAP, NW, KS>),
                                                hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               KS * BIAS_RING + 4 * BIAS_MAX_TABLE) == hipSuccess;
+                                               4 * BIAS_MAX_TABLE) == hipSuccess;
     if (!ok) fail("the kernel cannot have its LDS");
-    const size_t lds = KS * BIAS_RING + (BIAS == BIAS_TABLE ? 4 * (size_t)p.each * p.row : 0);
+    const size_t lds = BIAS == BIAS_TABLE ? 4 * (size_t)p.each * p.row : 0;
     hipLaunchKernelGGL((attn_bias_kernel<BF, BIAS, CAP, NW, KS>), dim3((unsigned)(tiles * p.chunks)), dim3(64 * NW * KS), lds, st, p);
 }
 
@@ -468,6 +466,7 @@ void attn_bias_launch(const AttnBias& a, const Scratch& s, hipStream_t st) {
         fail("the scratch has " + std::to_string(s.ws_floats) + " floats and " + std::to_string(s.n_counters) + " counters, not " +
              std::to_string(need.floats) + " and " + std::to_string(need.counters));
     BiasParams p = bias_params(a);
+    p.by_tiles = Div((uint32_t)(plan.tiles / a.kv_heads)), p.by_chunks = Div(plan.chunks);
     p.chunks = plan.chunks, p.ws = s.ws, p.counters = s.counters;
     const int bias = a.table ? BIAS_TABLE : a.slopes ? BIAS_SLOPES : BIAS_NONE;
     a.bf16 ? launch_type<true>(p, plan, bias, a.cap > 0.0f, st) : launch_type<false>(p, plan, bias, a.cap > 0.0f, st);

@@ -5,9 +5,9 @@
 // Two launches, each over the scores again (seven products in place of five), so that no block adds to
 // another's results and the gradients are the same bits at every call:
 // - dq_kernel: 16 NW queries of a head over their keys: dQ, the rows' constants for the other (-lse,
-//   -D, their keys) and the block's sums of dS by bucket.
-// - dkv_kernel: 16 NG NW keys of a key head over the queries that see them: dK and dV; further blocks
-//   sum the buckets' shares over the first launch's blocks.
+//   -D, their keys) and the block's sums of dS by distance.
+// - dkv_kernel: 16 NG NW keys of a key head over the queries that see them: dK and dV; its first blocks
+//   sum the distances' shares over the first launch's, and by bucket.
 //
 // - Both keep the scores where the next product wants them: a lane's column is its query (dQ) or its
 //   key (dK, dV), and the transposed operand comes from LDS by the transposing read.
@@ -21,7 +21,7 @@
 // - The bias's gradient in 32 bits, before dS is rounded: a 64-key block past `reach` on one side adds
 //   to one sum; else the 16 queries of a wave are summed along the diagonals with lane shifts (a
 //   lane's four keys of a 16-key tile against its neighbours' queries) and added to the wave's own
-//   row of distances in LDS, which the block sums by bucket at its end.
+//   row of distances in LDS.
 // - A row whose sums are not finite is computed again key by key over the pairs that are not masked: a
 //   masked infinity or NaN times a weight of 0 is NaN in the tile's products.
 #include <algorithm>
@@ -40,13 +40,14 @@ struct BiasBack {
     int64_t dq_stride, dkv_stride;
     float* dtable;
     // The workspace: per head and (padded) row -lse log2(e) (-inf: a row without keys) and -D, per row
-    // its keys (first, number), per 16 rows the keys (least first, most past last, most first, least
-    // past last) and a head's largest |dO|^2, per (head, block) the buckets' sums.
+    // its keys (first, number), per 16 NW rows the keys (least first, most past last, most first, least
+    // past last), per 16 rows a head's largest |dO|^2, per (head, block) the distances' sums.
     float *nl, *dn;
     int2* range;
     int4* bounds;
     float *max_do, *part;
     int nqp, tiles, dkv_blocks;  // tiles: a head's blocks of the first launch
+    int fine;                    // whether they have 16 rows (else 64)
 };
 
 constexpr int DQ_STAGE = 16384;           // K and V of 64 keys
@@ -97,28 +98,53 @@ __device__ __forceinline__ void sum_groups(int m, int n, float* sm, float* out, 
     }
 }
 
+// v by a DPP lane pattern in the 16-lane rows of ROWS (zero where the pattern leaves a row), `old` elsewhere.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_rows(float old, float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xF, true));
+}
+
+// Sums along the diagonals of a 16 x 16 tile S^T (lane (r16, g): query r16, keys 4 g + e): to here[i] of
+// lane x (any i, any lane group) the sum at distance (the tile's first key less its first query) - x, to
+// next[i] that at 16 more. First a lane's four keys against its neighbours' queries: key e of lane r16
+// is on the diagonal of key 0 of the lane e to the left, or 16 on where that leaves the 16 lanes. Then
+// the four groups of lanes, 4 g keys apart, by the same shift a group; an MFMA with ones adds the groups.
+__device__ __forceinline__ void diagonal_sums(floatx4 s, floatx4& here, floatx4& next) {
+    float a = s[0], b = dpp_move<0x11F>(s[1]);
+    a += dpp_move<0x101>(s[1]);
+    a += dpp_move<0x102>(s[2]);
+    a += dpp_move<0x103>(s[3]);
+    b += dpp_move<0x11E>(s[2]);
+    b += dpp_move<0x11D>(s[3]);
+    // lane x of group g from lane x + 4 g of its 16, and what leaves them, 16 further on (b's are the last
+    // three lanes: none of them leaves again)
+    auto left = [](float v) { return dpp_rows<0x10C, 8>(dpp_rows<0x108, 4>(dpp_rows<0x104, 2>(v, v), v), v); };
+    const float over = dpp_rows<0x114, 8>(dpp_rows<0x118, 4>(dpp_rows<0x11C, 2>(0.0f, a), a), a);
+    here = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, left(a), here, 0, 0, 0);
+    next = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, over + left(b), next, 0, 0, 0);
+}
+
 // ---- dQ of 16 NW queries of a head --------------------------------------------------------------
 template <bool BF, int BIAS, bool CAP, int NW, int KS>
 __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) {
     const BiasParams& p = b.p;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    // (stages: as in the forward pass, arrays of their own)
+    __shared__ __attribute__((aligned(16))) char stage0[KS * DQ_STAGE], stage1[KS * DQ_STAGE];
+    extern __shared__ __attribute__((aligned(16))) float tab0[];
     constexpr int QB = 16 * NW, LOADS = 16 / NW;
-    const int task = xcd_task(blockIdx.x, b.tiles * p.heads);
-    const int h = task / b.tiles, tile = task % b.tiles, q0 = QB * tile, kvh = h / p.each;
+    const Quotient ht = divide(xcd_task(blockIdx.x, gridDim.x), p.by_tiles);
+    const int h = ht.q, tile = ht.r, q0 = QB * tile, kvh = divide(h, p.by_each).q;
     const int tid = threadIdx.x, l = tid & 63, r16 = l & 15, g = l >> 4;
     const int wk = __builtin_amdgcn_readfirstlane(tid >> 6), w = wk % NW, kg = wk / NW;
     const int j4 = r16 >> 2, q4 = r16 & 3;
     const int dists = 2 * p.reach + 1;
-    char* const ring = lds + kg * 2 * DQ_STAGE;
-    float* const ring0 = (float*)lds;
-    float* const tab0 = (float*)(lds + KS * 2 * DQ_STAGE);
-    int* const bucket = (int*)(tab0 + p.row);
-    float* const hist0 = tab0 + p.row + dists;
+    float* const hist0 = tab0 + p.row;
     float* const hist = hist0 + wk * dists;
 
     // The keys of the block's rows (lane l: row q0 + l), then the lane's own row.
     KeyRange tr{0, 0};
-    if (l < QB && q0 + l < p.nq) tr = key_range(p, q0 + l);
+    const bool listed = l < QB && q0 + l < p.nq;
+    if (listed) tr = key_range(p, q0 + l);
     const int row = q0 + 16 * w + r16, qi = min(row, p.nq - 1), qpos = p.q_first + row;
     const bool real = row < p.nq;
     half8 qf[2], gf[2], of[2];
@@ -131,7 +157,8 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
             qf[k2] = *(const half8*)(qp + 32 * k2), gf[k2] = *(const half8*)(gp + 32 * k2), of[k2] = *(const half8*)(op + 32 * k2);
     }
     const float lse = p.lse[(size_t)h * p.nq + qi];
-    const int k0 = wave_min(tr.hi > tr.lo ? tr.lo : 0x7fffffff), k1 = wave_max(tr.hi);
+    const KeyBounds kb_ = key_bounds(tr, listed, w);
+    const int k0 = kb_.k0, k1 = kb_.k1, wlo = kb_.lo, whi = kb_.hi, flo = kb_.flo, fhi = kb_.fhi;
     const int nblk = k1 > k0 ? (k1 - k0 + 63) >> 6 : 0;
     uint32_t doff[LOADS];
 #pragma unroll
@@ -139,8 +166,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
         const int c = ((w + NW * x) & 7) * 64 + l, r = c >> 3, ch = (c & 7) ^ (r & 7);
         doff[x] = (uint32_t)(r * (int)p.kv_stride * 2 + ch * 16);
     }
-    auto stage = [&](int bl, int st) {
-        char* to = ring + st * DQ_STAGE;
+    auto stage = [&](int bl, char* to) {
         const int kb = k0 + 64 * bl;
         const uint32_t bytes = (uint32_t)((min(k1 - kb, 64) - 1) * (int)p.kv_stride * 2 + 128);
         const auto rk = buffer_rsrc(p.k + (int64_t)kb * p.kv_stride + kvh * 64, bytes);
@@ -150,9 +176,9 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
             lds_bdma16<false>(x < LOADS / 2 ? rk : rv, doff[x], to + (x < LOADS / 2 ? 0 : 8192) + ((w + NW * x) & 7) * 1024);
     };
     auto has = [&](int s) { return kg + KS * s < nblk; };
-    if (has(0)) stage(kg, 0);
+    if (has(0)) stage(kg, stage0 + kg * DQ_STAGE);
     if (BIAS == BIAS_TABLE) {
-        load_bias(p, h, 1, tab0, 64 * NW * KS, bucket);
+        load_bias(p, h, 1, tab0, 64 * NW * KS);
         for (int i = l; i < dists; i += 64) hist[i] = 0.0f;
     }
 
@@ -177,9 +203,6 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     const float dn = real ? -d : 0.0f;
     const float sigma = BF ? 1.0f : grad_scale(sq);
     const KeyRange kr = {__shfl(tr.lo, 16 * w + r16), __shfl(tr.hi, 16 * w + r16)};
-    const bool mine = (l >> 4) == w;
-    const int wlo = wave_min(mine && tr.hi > tr.lo ? tr.lo : 0x7fffffff), whi = wave_max(mine ? tr.hi : 0);
-    const int flo = wave_max(mine ? tr.lo : 0), fhi = wave_min(mine && q0 + l < p.nq ? tr.hi : 0x7fffffff);
     if (kg == 0) {
         if (g == 0) {
             b.nl[(size_t)h * b.nqp + row] = nl;
@@ -189,7 +212,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
         const float m = row_max(sq);
         if (l == 0) {
             b.max_do[(size_t)h * (b.nqp / 16) + q0 / 16 + w] = m;
-            if (h == 0) b.bounds[q0 / 16 + w] = make_int4(wlo, whi, flo, fhi);
+            if (h == 0 && w == 0) b.bounds[tile] = make_int4(k0, k1, kb_.all_flo, kb_.all_fhi);
         }
     }
     const int wq0 = p.q_first + q0 + 16 * w, wql = wq0 + 15;
@@ -211,26 +234,33 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     for (int t = 0; t < 4; t++) dq[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     auto step = [&](int s, auto st_) {
         constexpr int ST = decltype(st_)::value;
-        wait_vmcnt<0>();
-        __builtin_amdgcn_s_barrier();
-        const int kb = k0 + 64 * (kg + KS * s);
-        const bool act = has(s) && !(kb + 64 <= wlo || kb >= whi);
-        const char* st = ring + ST * DQ_STAGE;
-        floatx4 base[4], sc[4], ds[4];
-        half4 kt[2][4][2];
-        if (act) {
-            block_bias<BIAS>(p, tab, left, right, slope, kb, g, qpos, wq0, wql, base);
-            half8 kf[4][2], vf[4][2];
+        stage_barrier();
+        const int kb0 = k0 + 64 * (kg + KS * s);
+        const char* st = (ST ? stage1 : stage0) + kg * DQ_STAGE;
+        if (has(s + 1)) stage(kg + KS * (s + 1), (ST ? stage0 : stage1) + kg * DQ_STAGE);
+        if (!has(s) || kb0 + 64 <= wlo || kb0 >= whi) return;
+        floatx4 diag[3];  // sums along diagonals; those that run from one half's keys into the next's go on
+        if (BIAS == BIAS_TABLE) diag[0] = diag[1] = diag[2] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+        for (int hf = 0; hf < 2; hf++) {  // 32 keys: kb + 16 t + 4 g + e
+            const int kb = kb0 + 32 * hf;
+            floatx4 base[2], sc[2], ds[2];
+            half8 kf[2][2], vf[2][2];
+            half4 kt[4][2];
+            block_bias<BIAS>(p, tab, left, right, slope, kb, g, qpos, wq0, wql, base);
+#pragma unroll
+            for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int k2 = 0; k2 < 2; k2++) {
-                    kf[t][k2] = *(const half8*)(st + koff[k2] + 2048 * t);
-                    vf[t][k2] = *(const half8*)(st + 8192 + koff[k2] + 2048 * t);
+                    kf[t][k2] = *(const half8*)(st + koff[k2] + 4096 * hf + 2048 * t);
+                    vf[t][k2] = *(const half8*)(st + 8192 + koff[k2] + 4096 * hf + 2048 * t);
                 }
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
+            for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) kt[dt][y] = lds_read_tr16(st + toff[dt] + 4096 * hf + 2048 * y);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
                 sc[t] = CAP ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : base[t];
                 ds[t] = floatx4{dn, dn, dn, dn};
 #pragma unroll
@@ -238,84 +268,63 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
 #pragma unroll
                 for (int k2 = 0; k2 < 2; k2++) ds[t] = mma<BF>(vf[t][k2], gf[k2], ds[t]);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            if (CAP) cap_scores<2, true>(p, sc, base, sigma);
+            if (!(kb >= flo && kb + 32 <= fhi)) {
+                const int at = kb + 4 * g - kr.lo;
 #pragma unroll
-            for (int hf = 0; hf < 2; hf++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int dt = 0; dt < 4; dt++)
-#pragma unroll
-                    for (int y = 0; y < 2; y++) kt[hf][dt][y] = lds_read_tr16(st + toff[dt] + 4096 * hf + 2048 * y);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (has(s + 1)) stage(kg + KS * (s + 1), (ST + 1) % 2);
-        __builtin_amdgcn_sched_barrier(0);
-        if (!act) return;
-        if (CAP) cap_scores<4, true>(p, sc, base, sigma);
-        if (!(kb >= flo && kb + 64 <= fhi)) {
-            const int at = kb + 4 * g - kr.lo;
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool ok = (uint32_t)(at + 16 * t + e) < kspan;
-                    sc[t][e] = ok ? sc[t][e] : -INFINITY;
-                    ds[t][e] = ok ? ds[t][e] : 0.0f;
-                }
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) ds[t][e] *= fast_exp2(CAP ? sc[t][e] + nl : fmaf(sc[t][e], p.mul, nl));
-        if (BIAS == BIAS_TABLE) {
-            if (kb - wql >= p.reach || kb + 63 - wq0 <= -p.reach) {
-                float v = 0.0f;
-#pragma unroll
-                for (int t = 0; t < 4; t++) v += (ds[t][0] + ds[t][1]) + (ds[t][2] + ds[t][3]);
-                if (kb > wq0) far_right += v;
-                else far_left += v;
-            } else {
-                // diag[t], lane (r16, g): the sum at distance kb + 16 t + 4 g - (wq0 + r16). A lane's
-                // e-th key is at its query's distance + e, which is the diagonal of the lane e to the
-                // left: those that leave the 16 lanes belong to the next 16 keys' diagonals.
-                float diag[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    diag[t] += ds[t][0];
-                    diag[t] += dpp_move<0x101>(ds[t][1]);
-                    diag[t] += dpp_move<0x102>(ds[t][2]);
-                    diag[t] += dpp_move<0x103>(ds[t][3]);
-                    diag[t + 1] += dpp_move<0x11F>(ds[t][1]);
-                    diag[t + 1] += dpp_move<0x11E>(ds[t][2]);
-                    diag[t + 1] += dpp_move<0x11D>(ds[t][3]);
-                }
-#pragma unroll
-                for (int t = 0; t < 5; t++) {
-                    const int x = kb + 16 * t + 4 * g - qpos;
-                    far_left += x < -p.reach ? diag[t] : 0.0f;
-                    far_right += x > p.reach ? diag[t] : 0.0f;
-                    // (one group of 16 lanes after the other: distinct distances in each)
-#pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        if (g == y && x >= -p.reach && x <= p.reach) hist[x + p.reach] += diag[t];
-                        __builtin_amdgcn_wave_barrier();
+                    for (int e = 0; e < 4; e++) {
+                        const bool ok = (uint32_t)(at + 16 * t + e) < kspan;
+                        sc[t][e] = ok ? sc[t][e] : -INFINITY;
+                        ds[t][e] = ok ? ds[t][e] : 0.0f;
                     }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) ds[t][e] *= fast_exp2(CAP ? sc[t][e] + nl : fmaf(sc[t][e], p.mul, nl));
+            if (BIAS == BIAS_TABLE) {
+                const bool far = kb - wql >= p.reach || kb + 31 - wq0 <= -p.reach;
+                if (far) {
+                    const float v = ((ds[0][0] + ds[0][1]) + (ds[0][2] + ds[0][3])) + ((ds[1][0] + ds[1][1]) + (ds[1][2] + ds[1][3]));
+                    if (kb > wq0) far_right += v;
+                    else far_left += v;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 2; t++) diagonal_sums(ds[t], diag[t], diag[t + 1]);
+                }
+                if (!far || hf == 1) {
+                    const int x0 = kb - wq0 - r16;
+                    const bool within = kb - wql >= -p.reach && kb + 47 - wq0 <= p.reach;
+#pragma unroll
+                    for (int t = 0; t < 2 + hf; t++) {
+                        const int x = x0 + 16 * t;
+                        const float v = diag[t][0];
+                        if (within) {
+                            if (g == 0) __hip_atomic_fetch_add(hist + x + p.reach, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                        } else if (g == 0) {
+                            if (x < -p.reach) far_left += v;
+                            else if (x > p.reach) far_right += v;
+                            else __hip_atomic_fetch_add(hist + x + p.reach, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                        }
+                    }
+                    diag[0] = diag[2];
+                    diag[1] = diag[2] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
             }
-        }
-        if (CAP || !BF) {
+            if (CAP || !BF) {
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) ds[t][e] *= CAP ? base[t][e] : sigma;
-        }
-#pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-            const half8 sf = pack8<BF>(ds[2 * hf], ds[2 * hf + 1]);
+                    for (int e = 0; e < 4; e++) ds[t][e] *= CAP ? base[t][e] : sigma;
+            }
+            const half8 sf = pack8<BF>(ds[0], ds[1]);
 #pragma unroll
             for (int dt = 0; dt < 4; dt++) {
-                const half4 lo = kt[hf][dt][0], hi = kt[hf][dt][1];
-                const half8 kf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                dq[dt] = mma<BF>(kf, sf, dq[dt]);
+                const half4 lo = kt[dt][0], hi = kt[dt][1];
+                const half8 ka = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                dq[dt] = mma<BF>(ka, sf, dq[dt]);
             }
         }
     };
@@ -333,20 +342,17 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     }
     __syncthreads();
     if (BIAS == BIAS_TABLE) {
+        float* to = b.part + ((size_t)h * b.tiles + tile) * dists;
         for (int i = tid; i < dists; i += 64 * NW * KS) {
             float s = hist0[i];
 #pragma unroll
             for (int x = 1; x < NW * KS; x++) s += hist0[x * dists + i];
-            hist0[i] = s;
+            to[i] = s;
         }
-        __syncthreads();
-        sum_groups<64 * NW * KS>(p.buckets, dists, ring0, b.part + ((size_t)h * b.tiles + tile) * p.buckets, 1,
-                                 [&](int x, int i) { return bucket[i] == x ? hist0[i] : 0.0f; });
-        __syncthreads();  // (the ring is free again)
     }
     if (KS > 1) {
         if (kg > 0) {
-            float* mg = (float*)lds + ((kg - 1) * NW + w) * 16 * 64;
+            float* mg = (float*)stage0 + ((kg - 1) * NW + w) * 16 * 64;
 #pragma unroll
             for (int f = 0; f < 16; f++) mg[f * 64 + l] = dq[f >> 2][f & 3];
         }
@@ -354,7 +360,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
         if (kg > 0) return;
 #pragma unroll
         for (int k = 1; k < KS; k++) {
-            const float* mg = (const float*)lds + ((k - 1) * NW + w) * 16 * 64;
+            const float* mg = (const float*)stage0 + ((k - 1) * NW + w) * 16 * 64;
 #pragma unroll
             for (int f = 0; f < 16; f++) dq[f >> 2][f & 3] += mg[f * 64 + l];
         }
@@ -396,23 +402,27 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
 template <bool BF, int BIAS, bool CAP, int NG, int NW, int KS>
 __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b) {
     const BiasParams& p = b.p;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ __attribute__((aligned(16))) char stage0[KS * DKV_STAGE], stage1[KS * DKV_STAGE];
+    extern __shared__ __attribute__((aligned(16))) float tab0[];
     constexpr int WK = 16 * NG, KB = WK * NW, LOADS = 16 / NW;
-    if (BIAS == BIAS_TABLE && (int)blockIdx.x >= b.dkv_blocks) {
-        const int h = blockIdx.x - b.dkv_blocks;
-        const float* from = b.part + (size_t)h * b.tiles * p.buckets;
-        sum_groups<64 * NW * KS>(p.buckets, b.tiles, (float*)lds, b.dtable + h, p.heads,
-                                 [&](int x, int i) { return from[(size_t)i * p.buckets + x]; });
+    const int first = BIAS == BIAS_TABLE ? p.heads : 0;
+    if ((int)blockIdx.x < first) {  // (first, so that they are done long before the others)
+        const int h = blockIdx.x, dists = 2 * p.reach + 1;
+        const float* from = b.part + (size_t)h * b.tiles * dists;
+        float *sm = (float*)stage0, *sums = sm + 64 * NW * KS;
+        int* bucket = (int*)(sums + dists);
+        sum_groups<64 * NW * KS>(dists, b.tiles, sm, sums, 1, [&](int x, int i) { return from[(size_t)i * dists + x]; });
+        for (int i = threadIdx.x; i < dists; i += 64 * NW * KS) bucket[i] = min(max(p.bucket[i], 0), p.buckets - 1);
+        __syncthreads();
+        sum_groups<64 * NW * KS>(p.buckets, dists, sm, b.dtable + h, p.heads,
+                                 [&](int x, int i) { return bucket[i] == x ? sums[i] : 0.0f; });
         return;
     }
-    const int tiles = (p.nk + KB - 1) / KB;
-    const int task = xcd_task(blockIdx.x, b.dkv_blocks);
-    const int kvh = task / tiles, kb = (task % tiles) * KB;
+    const Quotient ht = divide(xcd_task(blockIdx.x - first, b.dkv_blocks), p.by_tiles);
+    const int kvh = ht.q, kb = ht.r * KB;
     const int tid = threadIdx.x, l = tid & 63, r16 = l & 15, g = l >> 4;
     const int wk = __builtin_amdgcn_readfirstlane(tid >> 6), w = wk % NW, kg = wk / NW;
     const int j4 = r16 >> 2, q4 = r16 & 3;
-    char* const ring = lds + kg * 2 * DKV_STAGE;
-    float* const tab0 = (float*)(lds + KS * 2 * DKV_STAGE);
     const int qt = b.nqp / 64;
 
     // This wave's keys: kw .. + WK - 1, the lane's the r16th of each 16.
@@ -430,31 +440,20 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
         }
     }
     if (BIAS == BIAS_TABLE) load_bias(p, kvh * p.each, p.each, tab0, 64 * NW * KS);
-    // 64 queries' keys, from those of 16
+    // 64 queries' keys
     auto tile_bounds = [&](int t) {
         int4 r = make_int4(0x7fffffff, 0, 0, 0x7fffffff);
-        if (t < qt)
+        if (t < qt) {
+            if (!b.fine) return b.bounds[t];
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 const int4 y = b.bounds[4 * t + x];
                 r.x = min(r.x, y.x), r.y = max(r.y, y.y), r.z = max(r.z, y.z), r.w = min(r.w, y.w);
             }
+        }
         return r;
     };
     float sigma = 1.0f;
-    if (!BF) {
-        float m = 0.0f;
-        for (int t = l; t < qt; t += 64) {
-            const int4 y = tile_bounds(t);
-            if (y.x < kb + KB && y.y > kb)
-                for (int s = 0; s < p.each; s++) {
-                    const floatx4 d = *(const floatx4*)(b.max_do + (size_t)(kvh * p.each + s) * (b.nqp / 16) + 4 * t);
-                    m = fmaxf(m, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])));
-                }
-        }
-        m = row_max(m);
-        sigma = grad_scale(max_xor32(max_xor16(m)));
-    }
 #pragma unroll
     for (int x = 0; x < NG; x++)
         if (key[x] >= p.nk) kf[x][0] = kf[x][1] = vf[x][0] = vf[x][1] = half8{};
@@ -470,8 +469,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
         const int c = ((w + NW * x) & 7) * 64 + l, r = c >> 3, ch = (c & 7) ^ (r & 7);
         off[x] = (uint32_t)(r * (int)(x < LOADS / 2 ? p.q_stride : b.do_stride) * 2 + ch * 16);
     }
-    auto stage = [&](int h, int t, int st) {
-        char* to = ring + st * DKV_STAGE;
+    auto stage = [&](int h, int t, char* to) {
         const int q0 = 64 * t, n = min(p.nq - q0, 64);
         const auto rq = buffer_rsrc(p.q + (int64_t)q0 * p.q_stride + h * 64, (uint32_t)((n - 1) * (int)p.q_stride * 2 + 128));
         const auto rg = buffer_rsrc(b.dout + (int64_t)q0 * b.do_stride + h * 64, (uint32_t)((n - 1) * (int)b.do_stride * 2 + 128));
@@ -494,10 +492,16 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
 #pragma unroll
     for (int dt = 0; dt < 4; dt++) toff[dt] = att_swz(4 * g + j4, 2 * dt + (q4 >> 1)) + (q4 & 1) * 8;
 
-    // 64 tiles of 64 queries at a time: those that see some of the block's keys, for each query head;
-    // group kg of the block takes every KS-th.
+    // 64 tiles of 64 queries at a time (the bounds of 256 loaded together): those that see some of the
+    // block's keys, for each query head; group kg of the block takes every KS-th.
+    int4 ahead[4];
     for (int t0 = 0; t0 < qt; t0 += 64) {
-        const int4 bd = tile_bounds(t0 + l);
+        if ((t0 & 255) == 0) {
+#pragma unroll
+            for (int x = 0; x < 4; x++) ahead[x] = tile_bounds(t0 + 64 * x + l);
+        }
+        const int4 bd = ahead[0];
+        ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
         const uint64_t seen = __builtin_amdgcn_ballot_w64(bd.x < kb + KB && bd.y > kb);
         if (seen == 0) continue;
         const int steps = p.each * __builtin_popcountll(seen);
@@ -513,13 +517,28 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
         skip(kg);
         int hx = sub, tx = t0 + __builtin_ctzll(rest);
         __syncthreads();  // the table; the stages of the last 64 tiles are no longer read
-        if (has(0)) stage(kvh * p.each + hx, tx, 0);
+        if (has(0)) stage(kvh * p.each + hx, tx, stage0 + kg * DKV_STAGE);
+        if (!BF) {
+            float m = 0.0f;
+            if ((seen >> l) & 1)
+                for (int s = 0; s < p.each; s++) {
+                    const floatx4 d = *(const floatx4*)(b.max_do + (size_t)(kvh * p.each + s) * (b.nqp / 16) + 4 * (t0 + l));
+                    m = fmaxf(m, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])));
+                }
+            const float was = sigma;
+            sigma = grad_scale(max_xor32(max_xor16(row_max(m))));
+            if (sigma != was) {
+#pragma unroll
+                for (int x = 0; x < NG; x++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) dk[x][t] = dk[x][t] * (sigma / was);
+            }
+        }
         auto step = [&](int s, auto st_) {
             constexpr int ST = decltype(st_)::value;
-            wait_vmcnt<0>();
-            __builtin_amdgcn_s_barrier();
+            stage_barrier();
             if (!has(s)) return;
-            const char* st = ring + ST * DKV_STAGE;
+            const char* st = (ST ? stage1 : stage0) + kg * DKV_STAGE;
             const int pos0 = p.q_first + 64 * tx, h = kvh * p.each + hx, at_t = tx - t0;
             const int lo = __builtin_amdgcn_readlane(bd.x, at_t), hi = __builtin_amdgcn_readlane(bd.y, at_t);
             const int flo = __builtin_amdgcn_readlane(bd.z, at_t), fhi = __builtin_amdgcn_readlane(bd.w, at_t);
@@ -529,15 +548,12 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
             const float* nl = (const float*)(st + 16384);
             const float* dn = (const float*)(st + 16384 + 256);
             const int2* rg = (const int2*)(st + 16384 + 512);
-            bool more = false;
             if (has(s + 1)) {
                 skip(KS);
-                hx = sub, tx = t0 + __builtin_ctzll(rest), more = true;
+                hx = sub, tx = t0 + __builtin_ctzll(rest);
+                stage(kvh * p.each + hx, tx, (ST ? stage0 : stage1) + kg * DKV_STAGE);
             }
-            if (!act) {
-                if (more) stage(kvh * p.each + hx, tx, (ST + 1) % 2);
-                return;
-            }
+            if (!act) return;
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {  // 32 queries: rows 32 hf + 16 t + 4 g + e of the tile, column key[x]
                 half8 qa[2][2], ga[2][2];
@@ -581,7 +597,6 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
 #pragma unroll
                     for (int y = 0; y < 2 * NG; y++) base[y] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
-                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int x = 0; x < NG; x++)
 #pragma unroll
@@ -617,11 +632,6 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
                         gt[dt][y] = lds_read_tr16(st + 8192 + toff[dt] + 4096 * hf + 2048 * y);
                         qt4[dt][y] = lds_read_tr16(st + toff[dt] + 4096 * hf + 2048 * y);
                     }
-                if (hf == 1) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (more) stage(kvh * p.each + hx, tx, (ST + 1) % 2);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
                 half8 pf[NG], sf[NG];
 #pragma unroll
                 for (int x = 0; x < NG; x++) {
@@ -659,7 +669,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
     if (KS > 1) {
         __syncthreads();
         if (kg > 0) {
-            float* mg = (float*)lds + ((kg - 1) * NW + w) * 32 * NG * 64;
+            float* mg = (float*)stage0 + ((kg - 1) * NW + w) * 32 * NG * 64;
 #pragma unroll
             for (int x = 0; x < NG; x++)
 #pragma unroll
@@ -672,7 +682,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
         if (kg > 0) return;
 #pragma unroll
         for (int k = 1; k < KS; k++) {
-            const float* mg = (const float*)lds + ((k - 1) * NW + w) * 32 * NG * 64;
+            const float* mg = (const float*)stage0 + ((k - 1) * NW + w) * 32 * NG * 64;
 #pragma unroll
             for (int x = 0; x < NG; x++)
 #pragma unroll
@@ -771,9 +781,9 @@ Layout layout(const AttnBias& a, const GradPlan& plan) {
         return at;
     };
     y.nl = take((size_t)a.heads * y.nqp), y.dn = take((size_t)a.heads * y.nqp);
-    y.range = take(2 * (size_t)y.nqp), y.bounds = take(4 * (size_t)(y.nqp / 16));
+    y.range = take(2 * (size_t)y.nqp), y.bounds = take(4 * (size_t)y.tiles);
     y.max_do = take((size_t)a.heads * (y.nqp / 16));
-    y.part = take(a.table ? (size_t)a.heads * y.tiles * a.buckets : 0);
+    y.part = take(a.table ? (size_t)a.heads * y.tiles * (2 * a.reach + 1) : 0);
     return y;
 }
 
@@ -785,23 +795,24 @@ bool lds_limit(K kernel, int bytes) {
 }
 
 template <bool BF, int BIAS, bool CAP, int NW, int KS>
-void launch_dq(const BiasBack& b, hipStream_t st) {
-    constexpr int ring = KS * 2 * DQ_STAGE, waves = NW * KS;
+void launch_dq(BiasBack b, hipStream_t st) {
+    constexpr int waves = NW * KS;
     static const bool ok = lds_limit(attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>,
-                                     ring + 4 * (bias_row(BIAS_MAX_REACH) + (waves + 1) * (2 * BIAS_MAX_REACH + 1)));
+                                     4 * (bias_row(BIAS_MAX_REACH) + waves * (2 * BIAS_MAX_REACH + 1)));
     (void)ok;
-    const size_t lds = ring + (BIAS == BIAS_TABLE ? 4 * (b.p.row + (waves + 1) * (2 * (size_t)b.p.reach + 1)) : 0);
+    const size_t lds = BIAS == BIAS_TABLE ? 4 * (b.p.row + waves * (2 * (size_t)b.p.reach + 1)) : 0;
+    b.p.by_tiles = Div(b.tiles);
     hipLaunchKernelGGL((attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>), dim3(b.tiles * b.p.heads), dim3(64 * waves), lds, st, b);
 }
 
 template <bool BF, int BIAS, bool CAP, int NG, int NW, int KS>
 void launch_dkv(BiasBack b, hipStream_t st) {
-    constexpr int ring = KS * 2 * DKV_STAGE;
-    static const bool ok = lds_limit(attn_bias_dkv_kernel<BF, BIAS, CAP, NG, NW, KS>, ring + 4 * BIAS_MAX_TABLE);
+    static const bool ok = lds_limit(attn_bias_dkv_kernel<BF, BIAS, CAP, NG, NW, KS>, 4 * BIAS_MAX_TABLE);
     (void)ok;
-    b.dkv_blocks = (b.p.nk + 16 * NG * NW - 1) / (16 * NG * NW) * b.p.kv_heads;
+    const int tiles = (b.p.nk + 16 * NG * NW - 1) / (16 * NG * NW);
+    b.dkv_blocks = tiles * b.p.kv_heads, b.p.by_tiles = Div(std::max(tiles, 1));
     const int blocks = b.dkv_blocks + (BIAS == BIAS_TABLE ? b.p.heads : 0);
-    const size_t lds = ring + (BIAS == BIAS_TABLE ? 4 * (size_t)b.p.each * b.p.row : 0);
+    const size_t lds = BIAS == BIAS_TABLE ? 4 * (size_t)b.p.each * b.p.row : 0;
     if (blocks) hipLaunchKernelGGL((attn_bias_dkv_kernel<BF, BIAS, CAP, NG, NW, KS>), dim3(blocks), dim3(64 * NW * KS), lds, st, b);
 }
 
@@ -833,7 +844,7 @@ void attn_bias_backward_launch(const AttnBias& a, const AttnBiasGrads& g, const 
     if (y.all > s.ws_floats) fail("the scratch has " + std::to_string(s.ws_floats) + " floats, not " + std::to_string(y.all));
     BiasBack b{};
     b.p = bias_params(a);
-    b.nqp = y.nqp, b.tiles = y.tiles;
+    b.nqp = y.nqp, b.tiles = y.tiles, b.fine = plan.dq_nw == 1;
     b.dout = (const f16*)g.dout, b.do_stride = g.do_stride;
     b.dq = (f16*)g.dq, b.dk = (f16*)g.dk, b.dv = (f16*)g.dv;
     b.dq_stride = g.dq_stride, b.dkv_stride = g.dkv_stride, b.dtable = g.dtable;

@@ -7,6 +7,22 @@
 
 namespace jh {
 
+// Division by a number that the host knows, in five operations (the compiler's takes some 30, and a
+// block does several before its first load): m = 2^32 / d rounded down, so the product's high word is
+// the quotient or one less.
+struct Div {
+    uint32_t d, m;
+    Div(uint32_t n = 1) : d(n), m(n > 1 ? (uint32_t)((uint64_t(1) << 32) / n) : 0xffffffffu) {}
+};
+struct Quotient {
+    int q, r;
+};
+__device__ __forceinline__ Quotient divide(int n, Div by) {
+    uint32_t q = __umulhi((uint32_t)n, by.m), r = (uint32_t)n - q * by.d;
+    if (r >= by.d) q++, r -= by.d;
+    return {(int)q, (int)r};
+}
+
 // What the kernels take: the attention in the units they work in. Scores run in the exp2 domain:
 // without a cap the MFMA accumulates q . k + (bias / scale), and a weight is exp2 of that times
 // `mul` = scale log2(e) less the row's log-sum; with one, a score is
@@ -21,6 +37,7 @@ struct BiasParams {
     f16* o;
     int64_t o_stride;
     int nq, nk, heads, kv_heads, each, q_first;
+    Div by_each, by_tiles, by_chunks;  // (by_tiles: the launch's tiles of a head)
     float scale, mul, unit, off, pre;
     float poly[5], small, per_off;  // (per_off: 1 / off)
     const float* table;
@@ -72,26 +89,29 @@ __device__ __forceinline__ float widen(f16 v) {
     return (float)v;
 }
 
-// The least and the most of a wave's values, to all lanes, without LDS (a shuffle's round trip is some
-// 100 clocks, and a block takes six such results before its first product): within 16 lanes by DPP,
-// as group_sum, then the lane swaps.
+// Least values without LDS (a shuffle's round trip is some 100 clocks, and a block takes several such
+// results before its first product): of each 16 lanes by DPP, as group_sum, and of the wave from
+// those by the lane swaps.
 template <int CTRL>
 __device__ __forceinline__ int dpp_int(int v) {
     return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
 }
-__device__ __forceinline__ int wave_min(int v) {
+__device__ __forceinline__ int row_min(int v) {
     v = min(v, dpp_int<0xB1>(v)), v = min(v, dpp_int<0x4E>(v));
-    v = min(v, dpp_int<0x141>(v)), v = min(v, dpp_int<0x140>(v));
+    v = min(v, dpp_int<0x141>(v));
+    return min(v, dpp_int<0x140>(v));
+}
+__device__ __forceinline__ int rows_min(int v) {
     const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     v = min((int)a[0], (int)a[1]);
     const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return __builtin_amdgcn_readfirstlane(min((int)b[0], (int)b[1]));
 }
-__device__ __forceinline__ int wave_max(int v) { return ~wave_min(~v); }
 // The most of 16 lanes' values, none negative, to each of them.
 __device__ __forceinline__ float row_max(float v) {
     v = fmaxf(v, dpp_move<0xB1>(v)), v = fmaxf(v, dpp_move<0x4E>(v));
-    return v = fmaxf(v, dpp_move<0x141>(v)), fmaxf(v, dpp_move<0x140>(v));
+    v = fmaxf(v, dpp_move<0x141>(v));
+    return fmaxf(v, dpp_move<0x140>(v));
 }
 
 // The keys that query i sees, [lo, hi) within [0, nk); none: lo = hi = 0.
@@ -111,6 +131,19 @@ __device__ __forceinline__ KeyRange key_range(const BiasParams& p, int i) {
     return hi > lo ? KeyRange{lo, hi} : KeyRange{0, 0};
 }
 
+// The keys of a block's rows, a lane each (`real`: it is a row): those that any of the block's or of wave
+// w's 16 sees lie in [k0, k1) or [lo, hi); every real row of the wave sees [flo, fhi), of the block
+// [all_flo, all_fhi).
+struct KeyBounds {
+    int k0, k1, lo, hi, flo, fhi, all_flo, all_fhi;
+};
+__device__ __forceinline__ KeyBounds key_bounds(KeyRange r, bool real, int w) {
+    const int a = row_min(r.hi > r.lo ? r.lo : 0x7fffffff), b = row_min(~r.hi);
+    const int c = row_min(~(real ? r.lo : 0)), d = row_min(real ? r.hi : 0x7fffffff);
+    return {rows_min(a), ~rows_min(b), __builtin_amdgcn_readlane(a, 16 * w), ~__builtin_amdgcn_readlane(b, 16 * w),
+            ~__builtin_amdgcn_readlane(c, 16 * w), __builtin_amdgcn_readlane(d, 16 * w), ~rows_min(c), rows_min(d)};
+}
+
 // A bias in the scores' units. A finite one stays finite: where every key
 // of a row has the lowest bias of the type, their weights are equal, as in the formula.
 __device__ __forceinline__ float bias_value(const BiasParams& p, float b) {
@@ -119,12 +152,11 @@ __device__ __forceinline__ float bias_value(const BiasParams& p, float b) {
 }
 
 // The padded distances of `n` heads from `head` on into LDS: tab[x row + reach + BIAS_PAD + t] is
-// the bias of head + x at distance t (key - query). bucket (nullable): the buckets of [-reach, reach].
-__device__ __forceinline__ void load_bias(const BiasParams& p, int head, int n, float* tab, int threads, int* bucket = nullptr) {
+// the bias of head + x at distance t (key - query).
+__device__ __forceinline__ void load_bias(const BiasParams& p, int head, int n, float* tab, int threads) {
     for (int i = threadIdx.x; i < p.row; i += threads) {
         const int t = min(max(i - BIAS_PAD, 0), 2 * p.reach);
         const int b = min(max(p.bucket[t], 0), p.buckets - 1);
-        if (bucket) bucket[t] = b;  // (the padding writes its end's again)
         for (int x = 0; x < n; x++) tab[x * p.row + i] = bias_value(p, p.table[(size_t)b * p.heads + head + x]);
     }
 }
@@ -197,33 +229,41 @@ __device__ __forceinline__ float bias_at(const BiasParams& p, const float* tab, 
     return 0.0f;
 }
 
-// The biases of a 64-key block from kb on for a lane's query (S^T: keys kb + 16 t + 4 g + e): tab, the
-// lane's distance 0; left, right: the table's ends; wq0, wql: the wave's first and last query.
-template <int BIAS>
+// The biases of 16 N keys from kb on for a lane's query (S^T: keys kb + 16 t + 4 g + e): tab, the lane's
+// distance 0; left, right: the table's ends; wq0, wql: the wave's first and last query.
+template <int BIAS, int N>
 __device__ __forceinline__ void block_bias(const BiasParams& p, const float* tab, float left, float right, float slope,
-                                           int kb, int g, int qpos, int wq0, int wql, floatx4 (&base)[4]) {
+                                           int kb, int g, int qpos, int wq0, int wql, floatx4 (&base)[N]) {
     if (BIAS == BIAS_TABLE) {
-        if (kb - wql >= p.reach || kb + 63 - wq0 <= -p.reach) {
+        if (kb - wql >= p.reach || kb + 16 * N - 1 - wq0 <= -p.reach) {
             const float b0 = kb > wq0 ? right : left;
 #pragma unroll
-            for (int t = 0; t < 4; t++) base[t] = floatx4{b0, b0, b0, b0};
+            for (int t = 0; t < N; t++) base[t] = floatx4{b0, b0, b0, b0};
         } else {
             const float* at = tab + (kb + 4 * g - qpos);
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int t = 0; t < N; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) base[t][e] = at[16 * t + e];
         }
     } else if (BIAS == BIAS_SLOPES) {
         const float x = (float)(kb + 4 * g - qpos);
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 0; t < N; t++)
 #pragma unroll
             for (int e = 0; e < 4; e++) base[t][e] = -slope * fabsf(x + (float)(16 * t + e));
     } else {
 #pragma unroll
-        for (int t = 0; t < 4; t++) base[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < N; t++) base[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+}
+
+// Before a step's reads: this wave's copies into LDS have landed (__syncthreads alone does not wait for
+// them, the wave's own reads of them do), then every wave's, and every wave's reads of the last step
+// are done.
+__device__ __forceinline__ void stage_barrier() {
+    wait_vmcnt<0>();
+    __syncthreads();
 }
 
 // Which of a wave's 16 rows (one a lane % 16) have a lane where `bad` holds.
