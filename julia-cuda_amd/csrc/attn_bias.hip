@@ -124,7 +124,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
     auto has = [&](int b) { return kg + KS * b < nblk; };
     auto step = [&](int b, auto st_) {
         constexpr int ST = decltype(st_)::value;
-        stage_barrier();
+        stage_barrier<0>();
         const int kb = k0 + 64 * (c0 + kg + KS * b);
         const bool act = has(b) && !(kb + 64 <= wlo || kb >= whi);
         const char* st = (ST ? stage1 : stage0) + kg * BIAS_STAGE;

@@ -39,11 +39,10 @@ struct BiasBack {
     f16 *dq, *dk, *dv;
     int64_t dq_stride, dkv_stride;
     float* dtable;
-    // The workspace: per head and (padded) row -lse log2(e) (-inf: a row without keys) and -D, per row
-    // its keys (first, number), per 16 NW rows the keys (least first, most past last, most first, least
+    // The workspace: per head and 64 (padded) rows -lse log2(e) (-inf: a row without keys), -D and the
+    // rows' keys (first, number), a kilobyte together (`info`); per 16 NW rows the keys (least first, most past last, most first, least
     // past last), per 16 rows a head's largest |dO|^2, per (head, block) the distances' sums.
-    float *nl, *dn;
-    int2* range;
+    float* info;
     int4* bounds;
     float *max_do, *part;
     int nqp, tiles, dkv_blocks;  // tiles: a head's blocks of the first launch
@@ -51,7 +50,12 @@ struct BiasBack {
 };
 
 constexpr int DQ_STAGE = 16384;           // K and V of 64 keys
-constexpr int DKV_STAGE = 16384 + 1024;   // Q, dO, -lse, -D and the key ranges of 64 queries
+constexpr int DKV_STAGE = 16384 + 1024;   // Q, dO and `info` of 64 queries
+
+// Row i of head h's -lse log2(e); its -D is 64 floats on, its keys at 128 + i % 64 more.
+__device__ __forceinline__ float* row_info(const BiasBack& b, int h, int i) {
+    return b.info + ((size_t)h * (b.nqp / 64) + (i >> 6)) * 256 + (i & 63);
+}
 
 // The power of two that takes the root of `sq` to between 2^3 and 2^4 (1 where it is 0 or not finite).
 __device__ __forceinline__ float grad_scale(float sq) {
@@ -205,9 +209,9 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     const KeyRange kr = {__shfl(tr.lo, 16 * w + r16), __shfl(tr.hi, 16 * w + r16)};
     if (kg == 0) {
         if (g == 0) {
-            b.nl[(size_t)h * b.nqp + row] = nl;
-            b.dn[(size_t)h * b.nqp + row] = dn;
-            if (h == 0) b.range[row] = make_int2(kr.lo, kr.hi - kr.lo);
+            float* to = row_info(b, h, row);
+            to[0] = nl, to[64] = dn;
+            *(int2*)(to + 128 + (row & 63)) = make_int2(kr.lo, kr.hi - kr.lo);
         }
         const float m = row_max(sq);
         if (l == 0) {
@@ -234,7 +238,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     for (int t = 0; t < 4; t++) dq[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     auto step = [&](int s, auto st_) {
         constexpr int ST = decltype(st_)::value;
-        stage_barrier();
+        stage_barrier<0>();
         const int kb0 = k0 + 64 * (kg + KS * s);
         const char* st = (ST ? stage1 : stage0) + kg * DQ_STAGE;
         if (has(s + 1)) stage(kg + KS * (s + 1), (ST ? stage0 : stage1) + kg * DQ_STAGE);
@@ -402,7 +406,12 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
 template <bool BF, int BIAS, bool CAP, int NG, int NW, int KS>
 __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b) {
     const BiasParams& p = b.p;
+    // Two stages, or three where the LDS has room: with two, a step waited for copies that it had seen
+    // issued only one step before (the batch's copies and barriers alone, without the products, took
+    // 51 of its 101 us).
+    constexpr int NS = KS == 1 ? 3 : 2;
     __shared__ __attribute__((aligned(16))) char stage0[KS * DKV_STAGE], stage1[KS * DKV_STAGE];
+    __shared__ __attribute__((aligned(16))) char stage2[NS == 3 ? KS * DKV_STAGE : 16];
     extern __shared__ __attribute__((aligned(16))) float tab0[];
     constexpr int WK = 16 * NG, KB = WK * NW, LOADS = 16 / NW;
     const int first = BIAS == BIAS_TABLE ? p.heads : 0;
@@ -473,18 +482,14 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
         const int q0 = 64 * t, n = min(p.nq - q0, 64);
         const auto rq = buffer_rsrc(p.q + (int64_t)q0 * p.q_stride + h * 64, (uint32_t)((n - 1) * (int)p.q_stride * 2 + 128));
         const auto rg = buffer_rsrc(b.dout + (int64_t)q0 * b.do_stride + h * 64, (uint32_t)((n - 1) * (int)b.do_stride * 2 + 128));
+        const auto ri = buffer_rsrc(b.info + ((size_t)h * qt + t) * 256, 1024);
 #pragma unroll
         for (int x = 0; x < LOADS; x++)
             lds_bdma16<false>(x < LOADS / 2 ? rq : rg, off[x], to + (x < LOADS / 2 ? 0 : 8192) + ((w + NW * x) & 7) * 1024);
 #pragma unroll
-        for (int x = 0; x < 4 / NW; x++) {  // -lse, -D and the two halves of the ranges, 256 bytes each
-            const int y = w + NW * x;
-            const void* src = y == 0 ? (const void*)(b.nl + (size_t)h * b.nqp + q0)
-                            : y == 1 ? (const void*)(b.dn + (size_t)h * b.nqp + q0)
-                                     : (const void*)((const int*)(b.range + q0) + 64 * (y - 2));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_rsrc(src, 256),
-                (__attribute__((address_space(3))) void*)(to + 16384 + 256 * y), 4, l * 4, 0, 0, 0);
-        }
+        for (int x = 0; x < 4 / NW; x++)  // (a quarter of `info` each)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                ri, (__attribute__((address_space(3))) void*)(to + 16384 + 256 * (w + NW * x)), 4, l * 4 + 256 * (w + NW * x), 0, 0, 0);
     };
     int aoff[2], toff[4];
 #pragma unroll
@@ -514,10 +519,19 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
             }
         };
         auto has = [&](int s) { return kg + KS * s < steps; };
+        struct Step {
+            int sub, t;
+        };
+        auto at_step = [&]() { return Step{sub, t0 + __builtin_ctzll(rest)}; };
         skip(kg);
-        int hx = sub, tx = t0 + __builtin_ctzll(rest);
+        Step now = at_step(), then = now;  // (then: the step after, of three stages)
         __syncthreads();  // the table; the stages of the last 64 tiles are no longer read
-        if (has(0)) stage(kvh * p.each + hx, tx, stage0 + kg * DKV_STAGE);
+        if (has(0)) stage(kvh * p.each + now.sub, now.t, stage0 + kg * DKV_STAGE);
+        if (NS == 3 && has(1)) {
+            skip(KS);
+            then = at_step();
+            stage(kvh * p.each + then.sub, then.t, stage1 + kg * DKV_STAGE);
+        }
         if (!BF) {
             float m = 0.0f;
             if ((seen >> l) & 1)
@@ -536,10 +550,12 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
         }
         auto step = [&](int s, auto st_) {
             constexpr int ST = decltype(st_)::value;
-            stage_barrier();
+            // (all but the next step's copies have landed)
+            if (NS == 3 && has(s + 1)) stage_barrier<NS == 3 ? LOADS + 4 / NW : 0>();
+            else stage_barrier<0>();
             if (!has(s)) return;
-            const char* st = (ST ? stage1 : stage0) + kg * DKV_STAGE;
-            const int pos0 = p.q_first + 64 * tx, h = kvh * p.each + hx, at_t = tx - t0;
+            const char* st = (ST == 0 ? stage0 : ST == 1 ? stage1 : stage2) + kg * DKV_STAGE;
+            const int hx = now.sub, pos0 = p.q_first + 64 * now.t, h = kvh * p.each + hx, at_t = now.t - t0;
             const int lo = __builtin_amdgcn_readlane(bd.x, at_t), hi = __builtin_amdgcn_readlane(bd.y, at_t);
             const int flo = __builtin_amdgcn_readlane(bd.z, at_t), fhi = __builtin_amdgcn_readlane(bd.w, at_t);
             const bool act = kw < hi && kw + WK > lo, full = kw >= flo && kw + WK <= fhi;
@@ -548,11 +564,14 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
             const float* nl = (const float*)(st + 16384);
             const float* dn = (const float*)(st + 16384 + 256);
             const int2* rg = (const int2*)(st + 16384 + 512);
-            if (has(s + 1)) {
+            now = then;
+            if (has(s + NS - 1)) {
                 skip(KS);
-                hx = sub, tx = t0 + __builtin_ctzll(rest);
-                stage(kvh * p.each + hx, tx, (ST ? stage0 : stage1) + kg * DKV_STAGE);
+                then = at_step();
+                constexpr int TO = (ST + NS - 1) % NS;
+                stage(kvh * p.each + then.sub, then.t, (TO == 0 ? stage0 : TO == 1 ? stage1 : stage2) + kg * DKV_STAGE);
             }
+            if (NS == 2) now = then;
             if (!act) return;
 #pragma unroll
             for (int hf = 0; hf < 2; hf++) {  // 32 queries: rows 32 hf + 16 t + 4 g + e of the tile, column key[x]
@@ -660,9 +679,10 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
             }
         };
         const int nsteps = (steps + KS - 1) / KS;
-        for (int s = 0; s < nsteps; s += 2) {
+        for (int s = 0; s < nsteps; s += NS) {
             step(s, std::integral_constant<int, 0>{});
             if (s + 1 < nsteps) step(s + 1, std::integral_constant<int, 1>{});
+            if (NS == 3 && s + 2 < nsteps) step(s + 2, std::integral_constant<int, NS - 1>{});
         }
     }
 
@@ -724,10 +744,10 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
                     float pw = 0.0f, da = 0.0f;
                     bool ok = false;
                     if (i < p.nq) {
-                        const int2 r = b.range[i];
+                        const float* of = row_info(b, h, i);
+                        const int2 r = *(const int2*)(of + 128 + (i & 63));
                         ok = (uint32_t)(j - r.x) < (uint32_t)r.y;
-                        const size_t at = (size_t)h * b.nqp + i;
-                        if (ok) grad_pair<BF, BIAS, CAP>(b, tab0 + sub * p.row, slope, h, kvh, i, j, b.nl[at], b.dn[at], pw, da);
+                        if (ok) grad_pair<BF, BIAS, CAP>(b, tab0 + sub * p.row, slope, h, kvh, i, j, of[0], of[64], pw, da);
                     }
                     uint64_t some = __builtin_amdgcn_ballot_w64(ok);
                     while (some) {
@@ -767,7 +787,7 @@ GradPlan grad_plan(const AttnBias& a, int cus) {
 
 // The workspace's parts, in floats, each on 256 bytes.
 struct Layout {
-    size_t nl, dn, range, bounds, max_do, part, all;
+    size_t info, bounds, max_do, part, all;
     int nqp, tiles;
 };
 
@@ -780,8 +800,7 @@ Layout layout(const AttnBias& a, const GradPlan& plan) {
         y.all += (floats + 63) / 64 * 64;
         return at;
     };
-    y.nl = take((size_t)a.heads * y.nqp), y.dn = take((size_t)a.heads * y.nqp);
-    y.range = take(2 * (size_t)y.nqp), y.bounds = take(4 * (size_t)y.tiles);
+    y.info = take(4 * (size_t)a.heads * y.nqp), y.bounds = take(4 * (size_t)y.tiles);
     y.max_do = take((size_t)a.heads * (y.nqp / 16));
     y.part = take(a.table ? (size_t)a.heads * y.tiles * (2 * a.reach + 1) : 0);
     return y;
@@ -848,7 +867,7 @@ void attn_bias_backward_launch(const AttnBias& a, const AttnBiasGrads& g, const 
     b.dout = (const f16*)g.dout, b.do_stride = g.do_stride;
     b.dq = (f16*)g.dq, b.dk = (f16*)g.dk, b.dv = (f16*)g.dv;
     b.dq_stride = g.dq_stride, b.dkv_stride = g.dkv_stride, b.dtable = g.dtable;
-    b.nl = s.ws + y.nl, b.dn = s.ws + y.dn, b.range = (int2*)(s.ws + y.range), b.bounds = (int4*)(s.ws + y.bounds);
+    b.info = s.ws + y.info, b.bounds = (int4*)(s.ws + y.bounds);
     b.max_do = s.ws + y.max_do, b.part = s.ws + y.part;
     const int bias = a.table ? BIAS_TABLE : a.slopes ? BIAS_SLOPES : BIAS_NONE;
     a.bf16 ? launch_type<true>(b, plan, bias, a.cap > 0.0f, st) : launch_type<false>(b, plan, bias, a.cap > 0.0f, st);

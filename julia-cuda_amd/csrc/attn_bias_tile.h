@@ -258,12 +258,16 @@ __device__ __forceinline__ void block_bias(const BiasParams& p, const float* tab
     }
 }
 
-// Before a step's reads: this wave's copies into LDS have landed (__syncthreads alone does not wait for
-// them, the wave's own reads of them do), then every wave's, and every wave's reads of the last step
-// are done.
+// Before a step's reads: all of this wave's copies into LDS but the last N have landed, then every
+// wave's, and every wave's reads of the last step are done. (__syncthreads waits for all copies, or for
+// none: its fence does not count them, only the wave's own reads of them do.)
+template <int N>
 __device__ __forceinline__ void stage_barrier() {
-    wait_vmcnt<0>();
-    __syncthreads();
+    static_assert(N >= 0 && N < 16, "vmcnt field");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(N | 0x0070);  // vmcnt N, lgkmcnt 0
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // Which of a wave's 16 rows (one a lane % 16) have a lane where `bad` holds.
