@@ -415,10 +415,16 @@ struct BiasPlan {
     long tiles;
 };
 
+// Key groups while the grid is small (MI355X, d = 768, us; nw x ks): 293 rows 1x4 6.2, 2x4 6.4; 448 rows
+// 2x4 6.9, 4x4 8.3, 4x1 9.0; 600 rows 2x4 8.2; 1024 rows 4x4 12.4, 4x2 13.5, 4x1 16.3; 2029 rows 4x2 33.4,
+// 4x1 36.4; 2900 rows 4x1 56.7, 4x2 62.7. One row over 8192 keys: a block for every 256 keys.
 BiasPlan bias_plan(const AttnBias& a, int cus) {
     const long rows = (long)a.nq * (a.heads / a.kv_heads);
-    const long t16 = (rows + 15) / 16 * a.kv_heads, t64 = (rows + 63) / 64 * a.kv_heads;
-    if (t16 > cus) return {4, 1, 1, t64};
+    const long t16 = (rows + 15) / 16 * a.kv_heads, t32 = (rows + 31) / 32 * a.kv_heads, t64 = (rows + 63) / 64 * a.kv_heads;
+    if (t16 > cus) {
+        if (t32 <= cus) return {2, 4, 1, t32};
+        return {4, t64 <= cus ? 4 : t64 <= 2L * cus ? 2 : 1, 1, t64};
+    }
     // a block for every 256 keys at most
     const long most = std::max(1L, std::min((long)(a.nk + 255) / 256, (long)cus / std::max(1L, t16)));
     return {1, 4, (int)most, t16};
@@ -437,6 +443,9 @@ void launch_tile(const BiasParams& p, long tiles, hipStream_t st) {
 template <bool BF, int BIAS, bool CAP>
 void launch_plan(const BiasParams& p, const BiasPlan& plan, hipStream_t st) {
     if (plan.nw == 1) launch_tile<BF, BIAS, CAP, 1, 4>(p, plan.tiles, st);
+    else if (plan.nw == 2) launch_tile<BF, BIAS, CAP, 2, 4>(p, plan.tiles, st);
+    else if (plan.ks == 4) launch_tile<BF, BIAS, CAP, 4, 4>(p, plan.tiles, st);
+    else if (plan.ks == 2) launch_tile<BF, BIAS, CAP, 4, 2>(p, plan.tiles, st);
     else launch_tile<BF, BIAS, CAP, 4, 1>(p, plan.tiles, st);
 }
 

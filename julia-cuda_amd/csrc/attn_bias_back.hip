@@ -46,7 +46,7 @@ struct BiasBack {
     int4* bounds;
     float *max_do, *part;
     int nqp, tiles, dkv_blocks;  // tiles: a head's blocks of the first launch
-    int fine;                    // whether they have 16 rows (else 64)
+    int per;                     // of them to 64 rows: 4, 2 or 1
 };
 
 constexpr int DQ_STAGE = 16384;           // K and V of 64 keys
@@ -453,10 +453,9 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
     auto tile_bounds = [&](int t) {
         int4 r = make_int4(0x7fffffff, 0, 0, 0x7fffffff);
         if (t < qt) {
-            if (!b.fine) return b.bounds[t];
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int4 y = b.bounds[4 * t + x];
+            if (b.per == 1) return b.bounds[t];
+            for (int x = 0; x < b.per; x++) {
+                const int4 y = b.bounds[b.per * t + x];
                 r.x = min(r.x, y.x), r.y = max(r.y, y.y), r.z = max(r.z, y.z), r.w = min(r.w, y.w);
             }
         }
@@ -770,18 +769,35 @@ namespace {
 
 [[noreturn]] void fail(const std::string& m) { throw std::runtime_error("attention_bias_backward: " + m); }
 
-// The tiles of a call: 16 nw queries or 16 ng nw keys a block, ks groups.
+constexpr int LDS_BYTES = 160 * 1024;
+
+// The tiles of a call: 16 dq_nw queries, 16 ng nw keys a block, in ks groups.
 struct GradPlan {
-    int dq_nw, dkv_ng, dkv_nw, dkv_ks;
+    int dq_nw, dq_ks, ng, nw, ks;
 };
 
+// More groups to a block, and smaller blocks, while the grid is about a block a CU or less (MI355X, d =
+// 768, us for the whole pass with the other launch as it is; nw x ks for dQ, ng x nw x ks for dK and dV):
+//    448 rows  dQ 2x4 20.3, 4x1 25.1, 1x4 26.2             dK, dV 1x2x4 25.2, 1x4x2 27.5, 2x4x1 33.2
+//   1024 rows  dQ 4x2 45.8, 4x4 46.9, 4x1 52.8             dK, dV 2x2x4 45.5, 1x4x2 47.1, 2x4x1 59.0
+//   1345 rows  dQ 4x1 86.0, 4x2 89.7                       dK, dV 2x4x2 74.1, 2x2x4 81.7, 2x4x1 85.4
+//   2029 rows  dQ 4x1 120, 4x2 123                         dK, dV 2x4x2 102, 2x2x4 111, 2x4x1 120
+//   2029 rows, prefix, capped, 4 key heads: dQ 4x2 115, 4x1 126;  dK, dV 1x2x4 128, 2x2x4 154, 2x4x1 286
+//   64 documents in 18752 rows: dQ 4x1 203, 4x2 264        dK, dV 2x4x1 205, 1x4x1 234, 2x4x2 241
+// (dQ's groups each need a row of distances to the table's reach in LDS.)
 GradPlan grad_plan(const AttnBias& a, int cus) {
-    const long q16 = (long)(a.nq + 15) / 16 * a.heads;
+    const long q16 = (long)(a.nq + 15) / 16 * a.heads, q32 = (long)(a.nq + 31) / 32 * a.heads, q64 = (long)(a.nq + 63) / 64 * a.heads;
     const long k16 = (long)(a.nk + 15) / 16 * a.kv_heads;
-    GradPlan y{4, 2, 4, 1};
-    if (q16 <= cus) y.dq_nw = 1;
-    if (k16 <= cus) y.dkv_ng = 1, y.dkv_nw = 1, y.dkv_ks = 4;
-    else if (k16 <= 4 * cus) y.dkv_ng = 1, y.dkv_nw = 2, y.dkv_ks = 4;
+    GradPlan y{4, 1, 2, 4, 1};
+    const long hist = a.table ? 4L * (bias_row(a.reach) + 8 * (2 * a.reach + 1)) : 0;  // of eight waves
+    const bool room = 8 * DQ_STAGE + hist <= LDS_BYTES;
+    if (q16 <= cus) y.dq_nw = 1, y.dq_ks = 4;
+    else if (q32 <= cus && room) y.dq_nw = 2, y.dq_ks = 4;
+    else if (2 * q64 <= 3L * cus) y.dq_ks = 2;
+    if (k16 <= cus) y.ng = 1, y.nw = 1, y.ks = 4;
+    else if (k16 <= 2L * cus) y.ng = 1, y.nw = 2, y.ks = 4;
+    else if (k16 <= 3L * cus) y.nw = 2, y.ks = 4;
+    else if (k16 <= 8L * cus) y.ks = 2;
     return y;
 }
 
@@ -817,7 +833,7 @@ template <bool BF, int BIAS, bool CAP, int NW, int KS>
 void launch_dq(BiasBack b, hipStream_t st) {
     constexpr int waves = NW * KS;
     static const bool ok = lds_limit(attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>,
-                                     4 * (bias_row(BIAS_MAX_REACH) + waves * (2 * BIAS_MAX_REACH + 1)));
+                                     std::min(4 * (bias_row(BIAS_MAX_REACH) + waves * (2 * BIAS_MAX_REACH + 1)), LDS_BYTES - 2 * KS * DQ_STAGE));
     (void)ok;
     const size_t lds = BIAS == BIAS_TABLE ? 4 * (b.p.row + waves * (2 * (size_t)b.p.reach + 1)) : 0;
     b.p.by_tiles = Div(b.tiles);
@@ -837,9 +853,16 @@ void launch_dkv(BiasBack b, hipStream_t st) {
 
 template <bool BF, int BIAS, bool CAP>
 void launch(const BiasBack& b, const GradPlan& plan, hipStream_t st) {
-    if (b.p.nq > 0) plan.dq_nw == 1 ? launch_dq<BF, BIAS, CAP, 1, 4>(b, st) : launch_dq<BF, BIAS, CAP, 4, 1>(b, st);
-    if (plan.dkv_nw == 1) launch_dkv<BF, BIAS, CAP, 1, 1, 4>(b, st);
-    else if (plan.dkv_nw == 2) launch_dkv<BF, BIAS, CAP, 1, 2, 4>(b, st);
+    if (b.p.nq > 0) {
+        if (plan.dq_nw == 1) launch_dq<BF, BIAS, CAP, 1, 4>(b, st);
+        else if (plan.dq_nw == 2) launch_dq<BF, BIAS, CAP, 2, 4>(b, st);
+        else if (plan.dq_ks == 2) launch_dq<BF, BIAS, CAP, 4, 2>(b, st);
+        else launch_dq<BF, BIAS, CAP, 4, 1>(b, st);
+    }
+    if (plan.nw == 1) launch_dkv<BF, BIAS, CAP, 1, 1, 4>(b, st);
+    else if (plan.ng == 1) launch_dkv<BF, BIAS, CAP, 1, 2, 4>(b, st);
+    else if (plan.nw == 2) launch_dkv<BF, BIAS, CAP, 2, 2, 4>(b, st);
+    else if (plan.ks == 2) launch_dkv<BF, BIAS, CAP, 2, 4, 2>(b, st);
     else launch_dkv<BF, BIAS, CAP, 2, 4, 1>(b, st);
 }
 
@@ -863,7 +886,7 @@ void attn_bias_backward_launch(const AttnBias& a, const AttnBiasGrads& g, const 
     if (y.all > s.ws_floats) fail("the scratch has " + std::to_string(s.ws_floats) + " floats, not " + std::to_string(y.all));
     BiasBack b{};
     b.p = bias_params(a);
-    b.nqp = y.nqp, b.tiles = y.tiles, b.fine = plan.dq_nw == 1;
+    b.nqp = y.nqp, b.tiles = y.tiles, b.per = 4 / plan.dq_nw;
     b.dout = (const f16*)g.dout, b.do_stride = g.do_stride;
     b.dq = (f16*)g.dq, b.dk = (f16*)g.dk, b.dv = (f16*)g.dv;
     b.dq_stride = g.dq_stride, b.dkv_stride = g.dkv_stride, b.dtable = g.dtable;

@@ -197,6 +197,9 @@ __device__ __forceinline__ void cap_scores(const BiasParams& p, floatx4 (&sc)[N]
                 }
             }
     } else {
+        // (opaque, or the compiler computes this side ahead of the branch every time)
+#pragma unroll
+        for (int t = 0; t < N; t++) asm volatile("" : "+v"(sc[t]));
 #pragma unroll
         for (int t = 0; t < N; t++)
 #pragma unroll

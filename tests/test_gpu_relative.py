@@ -162,6 +162,8 @@ CASES = [
     dict(type="f16", nq=1500, heads=4, bias="table", lens=[1500], prefix=[500]),
     dict(type="f16", nq=1400, heads=12, bias="table", lens=[300, 64, 500, 536]),
     dict(type="bf16", nq=1100, heads=16, bias="slopes", cap=30.0, lens=[1100], prefix=[100]),
+    dict(type="f16", nq=2100, heads=16, bias="table", lens=[700, 64, 5, 800, 531]),
+    dict(type="f16", nq=1000, heads=12, bias="table", reach=512),
 ]
 
 
