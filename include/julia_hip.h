@@ -260,14 +260,14 @@ int julia_hip_layer_norm(int type, const void *x, int64_t x_stride, int rows, in
                          const float *gamma, const float *beta, float eps, void *y,
                          int64_t y_stride, float *stats, void *stream, char *err, size_t err_len);
 /* Its gradients: dx in `type` (may be dy or x), dgamma and dbeta (nullable) [d] f32, summed over the
- * rows in a fixed order; all written, not added to. The scratch: julia_hip_layer_norm_scratch (no
- * counters). */
+ * rows in a fixed order; all written, not added to. The scratch: julia_hip_layer_norm_scratch. */
 int julia_hip_layer_norm_backward(int type, const void *x, int64_t x_stride, const void *dy,
                                   int64_t dy_stride, int rows, int d, const float *gamma,
                                   const float *stats, void *dx, int64_t dx_stride, float *dgamma,
                                   float *dbeta, const julia_hip_scratch *s, void *stream, char *err,
                                   size_t err_len);
-int julia_hip_layer_norm_scratch(int rows, int d, size_t *ws_floats, char *err, size_t err_len);
+int julia_hip_layer_norm_scratch(int rows, int d, size_t *ws_floats, size_t *counters, char *err,
+                                 size_t err_len);
 
 /* src/timing.rs:43-74 `timing::time` for one GEMM: `warmup` calls, then `batches` batches of
  * `per_batch` back-to-back calls between HIP events; min and median microseconds per call. */

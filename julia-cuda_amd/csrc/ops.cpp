@@ -92,10 +92,11 @@ int julia_hip_layer_norm(int type, const void* x, int64_t x_stride, int rows, in
     });
 }
 
-int julia_hip_layer_norm_scratch(int rows, int d, size_t* ws_floats, char* err, size_t err_len) {
+int julia_hip_layer_norm_scratch(int rows, int d, size_t* ws_floats, size_t* counters, char* err, size_t err_len) {
     return guarded(err, err_len, [&] {
-        if (!ws_floats) throw std::runtime_error("layer_norm: nowhere to put the size");
-        *ws_floats = norm_scratch(rows, d, device_cus()).floats;
+        if (!ws_floats || !counters) throw std::runtime_error("layer_norm: nowhere to put the sizes");
+        const ScratchSize s = norm_scratch(rows, d, device_cus());
+        *ws_floats = s.floats, *counters = s.counters;
     });
 }
 

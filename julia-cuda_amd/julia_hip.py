@@ -229,7 +229,8 @@ def lib():
         "julia_hip_layer_norm_backward": (_I, [_I, _VP, ctypes.c_int64, _VP, ctypes.c_int64, _I, _I,
                                                _VP, _VP, _VP, ctypes.c_int64, _VP, _VP, _VP, _VP,
                                                _CP, _SZ]),
-        "julia_hip_layer_norm_scratch": (_I, [_I, _I, ctypes.POINTER(_SZ), _CP, _SZ]),
+        "julia_hip_layer_norm_scratch": (_I, [_I, _I, ctypes.POINTER(_SZ), ctypes.POINTER(_SZ), _CP,
+                                              _SZ]),
         "julia_hip_prep_relative_buckets": (_I, [_I, _I, _I, _I, _I32P, _CP, _SZ]),
         "julia_hip_prep_spans": (_I, [_VP, _VP, _SZ, _VP, _CP, _SZ]),
         "julia_hip_encode_batch_phases": (_I, [_VP, _SZ, _VP, _VP, ctypes.POINTER(_F), _CP, _SZ]),
@@ -633,9 +634,9 @@ def layer_norm(type, x, rows, d, gamma, beta, eps, y, x_stride=0, y_stride=0, st
 
 def layer_norm_scratch(rows, d):
     """(ws_floats, counters) of the Scratch that layer_norm_backward takes."""
-    ws = ctypes.c_size_t()
-    _call(lib().julia_hip_layer_norm_scratch, rows, d, ctypes.byref(ws))
-    return ws.value, 0
+    ws, counters = ctypes.c_size_t(), ctypes.c_size_t()
+    _call(lib().julia_hip_layer_norm_scratch, rows, d, ctypes.byref(ws), ctypes.byref(counters))
+    return ws.value, counters.value
 
 
 def layer_norm_backward(type, x, dy, rows, d, gamma, stats, dx, dgamma, dbeta=0, x_stride=0,
