@@ -21,6 +21,7 @@
 namespace jh {
 
 constexpr int BIAS_STAGE = 16384;  // 64 keys: K, then V
+constexpr int BIAS_CHUNKS = 16;    // blocks that share a tile's keys, at most
 
 // The row's output again, key by key over the keys it sees: a masked key's V may hold infinities
 // or NaN, which a weight of 0 in the tile's product would turn into NaN for rows that do not see it.
@@ -257,14 +258,22 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
             }
     };
     merge_groups();
-    if (p.chunks > 1) {
-        float* const slots = p.ws + (size_t)tile * p.chunks * 18 * 64 * NW;
+    if (NW == 1 && p.chunks > 1) {
+        // A chunk's part: a lane's outputs as four 16-byte pieces, its maximum and its sum; the lanes of rows
+        // that there are. The last block's waves load all of their chunks' parts at once.
+        constexpr uint32_t PART = 18 * 64 * NW * 4;
+        constexpr int AT_ONCE = BIAS_CHUNKS / KS;
+        const auto slots = buffer_rsrc(p.ws + (size_t)tile * p.chunks * (PART / 4), PART * p.chunks);
+        const uint32_t lane16 = (w * 64 + l) * 16, lane8 = 64 * NW * 64 + (w * 64 + l) * 8;
+        const bool real = row < rows;
         if (kg == 0) {
-            float* to = slots + (size_t)chunk * 18 * 64 * NW + tid;
+            if (real) {
+                const uint32_t at = PART * chunk;
 #pragma unroll
-            for (int f = 0; f < 16; f++) xstore32(to + f * 64 * NW, o[f >> 2][f & 3]);
-            xstore32(to + 16 * 64 * NW, mx);
-            xstore32(to + 17 * 64 * NW, sum);
+                for (int dt = 0; dt < 4; dt++)
+                    bstore16f(slots, at + dt * 1024 * NW + lane16, make_float4(o[dt][0], o[dt][1], o[dt][2], o[dt][3]));
+                bstore8(slots, at + lane8, make_float2(mx, sum));
+            }
             release_wait();
         }
         __syncthreads();
@@ -278,13 +287,26 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
         mx = -INFINITY, sum = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < 4; dt++) o[dt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int z = kg; z < p.chunks; z += KS) {
-            const float* from = slots + (size_t)z * 18 * 64 * NW + w * 64 + l;
-            floatx4 ok[4];
+        if (real)
+            for (int z = kg; z < p.chunks; z += AT_ONCE * KS) {
+                float4 part[AT_ONCE][4];
+                float2 ms[AT_ONCE];
 #pragma unroll
-            for (int f = 0; f < 16; f++) ok[f >> 2][f & 3] = xload32(from + f * 64 * NW);
-            merge(xload32(from + 16 * 64 * NW), xload32(from + 17 * 64 * NW), ok);
-        }
+                for (int x = 0; x < AT_ONCE; x++) {
+                    const uint32_t at = PART * min(z + x * KS, p.chunks - 1);
+#pragma unroll
+                    for (int dt = 0; dt < 4; dt++) part[x][dt] = bload16f(slots, at + dt * 1024 * NW + lane16);
+                    ms[x] = bload8<true>(slots, at + lane8);
+                }
+#pragma unroll
+                for (int x = 0; x < AT_ONCE; x++) {
+                    if (z + x * KS >= p.chunks) break;
+                    floatx4 ok[4];
+#pragma unroll
+                    for (int dt = 0; dt < 4; dt++) ok[dt] = floatx4{part[x][dt].x, part[x][dt].y, part[x][dt].z, part[x][dt].w};
+                    merge(ms[x].x, ms[x].y, ok);
+                }
+            }
         merge_groups();
     }
     if (kg > 0) return;
@@ -417,7 +439,7 @@ struct BiasPlan {
 
 // Key groups while the grid is small (MI355X, d = 768, us; nw x ks): 293 rows 1x4 6.2, 2x4 6.4; 448 rows
 // 2x4 6.9, 4x4 8.3, 4x1 9.0; 600 rows 2x4 8.2; 1024 rows 4x4 12.4, 4x2 13.5, 4x1 16.3; 2029 rows 4x2 33.4,
-// 4x1 36.4; 2900 rows 4x1 56.7, 4x2 62.7. One row over 8192 keys: a block for every 256 keys.
+// 4x1 36.4; 2900 rows 4x1 56.7, 4x2 62.7.
 BiasPlan bias_plan(const AttnBias& a, int cus) {
     const long rows = (long)a.nq * (a.heads / a.kv_heads);
     const long t16 = (rows + 15) / 16 * a.kv_heads, t32 = (rows + 31) / 32 * a.kv_heads, t64 = (rows + 63) / 64 * a.kv_heads;
@@ -425,8 +447,10 @@ BiasPlan bias_plan(const AttnBias& a, int cus) {
         if (t32 <= cus) return {2, 4, 1, t32};
         return {4, t64 <= cus ? 4 : t64 <= 2L * cus ? 2 : 1, 1, t64};
     }
-    // a block for every 256 keys at most
-    const long most = std::max(1L, std::min((long)(a.nk + 255) / 256, (long)cus / std::max(1L, t16)));
+    // a block for every 256 keys at most, and few enough that their arrivals at the tile's counter, one
+    // after the other, cost less than their keys (one row, 4 key heads: 8192 keys in 32 chunks 11.9 us, in
+    // 16 9.6, in 8 11.0; 16384 keys in 64 16.8, in 32 12.3, in 16 12.0)
+    const long most = std::max(1L, std::min({(a.nk + 255L) / 256, (long)cus / std::max(1L, t16), (long)BIAS_CHUNKS}));
     return {1, 4, (int)most, t16};
 }
 
