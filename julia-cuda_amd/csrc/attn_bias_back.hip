@@ -20,8 +20,9 @@
 //   the grid is small; their sums join in LDS in order.
 // - The bias's gradient in 32 bits, before dS is rounded: a 64-key block past `reach` on one side adds
 //   to one sum; else the 16 queries of a wave are summed along the diagonals with lane shifts (a
-//   lane's four keys of a 16-key tile against its neighbours' queries) and added to the wave's own
-//   row of distances in LDS.
+//   lane's four keys of a 16-key tile against its neighbours' queries) and added to rows of distances
+//   in LDS that no other lane group adds to (64 documents in 18752 rows: dQ alone 61 us; with the sums
+//   on masked additions 128, the groups joined by shifts and an MFMA with ones 110, so 104).
 // - A row whose sums are not finite is computed again key by key over the pairs that are not masked: a
 //   masked infinity or NaN times a weight of 0 is NaN in the tile's products.
 #include <algorithm>
@@ -50,6 +51,14 @@ struct BiasBack {
 };
 
 constexpr int DQ_STAGE = 16384;           // K and V of 64 keys
+// The distances' sums in LDS: a row (and a spare) for each of a wave's four lane groups, so that no two lanes
+// share a sum (rows a multiple of 64 and 12 apart: with the groups' 4 keys, on different banks); a row a
+// wave for eight waves of four stages.
+__host__ __device__ constexpr int hist_groups(int nw) { return nw == 2 ? 1 : 4; }
+__host__ __device__ constexpr int hist_pitch(int reach) { return (2 * reach + 2 - 12 + 63) / 64 * 64 + 12; }
+__host__ __device__ constexpr int dq_lds(int reach, int nw, int ks) {  // beside the stages
+    return 4 * (2 * (reach + BIAS_PAD) + 1 + nw * ks * hist_groups(nw) * hist_pitch(reach));
+}
 constexpr int DKV_STAGE = 16384 + 1024;   // Q, dO and `info` of 64 queries
 
 // Row i of head h's -lse log2(e); its -D is 64 floats on, its keys at 128 + i % 64 more.
@@ -102,30 +111,18 @@ __device__ __forceinline__ void sum_groups(int m, int n, float* sm, float* out, 
     }
 }
 
-// v by a DPP lane pattern in the 16-lane rows of ROWS (zero where the pattern leaves a row), `old` elsewhere.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp_rows(float old, float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(v), CTRL, ROWS, 0xF, true));
-}
-
-// Sums along the diagonals of a 16 x 16 tile S^T (lane (r16, g): query r16, keys 4 g + e): to here[i] of
-// lane x (any i, any lane group) the sum at distance (the tile's first key less its first query) - x, to
-// next[i] that at 16 more. First a lane's four keys against its neighbours' queries: key e of lane r16
-// is on the diagonal of key 0 of the lane e to the left, or 16 on where that leaves the 16 lanes. Then
-// the four groups of lanes, 4 g keys apart, by the same shift a group; an MFMA with ones adds the groups.
-__device__ __forceinline__ void diagonal_sums(floatx4 s, floatx4& here, floatx4& next) {
-    float a = s[0], b = dpp_move<0x11F>(s[1]);
-    a += dpp_move<0x101>(s[1]);
-    a += dpp_move<0x102>(s[2]);
-    a += dpp_move<0x103>(s[3]);
-    b += dpp_move<0x11E>(s[2]);
-    b += dpp_move<0x11D>(s[3]);
-    // lane x of group g from lane x + 4 g of its 16, and what leaves them, 16 further on (b's are the last
-    // three lanes: none of them leaves again)
-    auto left = [](float v) { return dpp_rows<0x10C, 8>(dpp_rows<0x108, 4>(dpp_rows<0x104, 2>(v, v), v), v); };
-    const float over = dpp_rows<0x114, 8>(dpp_rows<0x118, 4>(dpp_rows<0x11C, 2>(0.0f, a), a), a);
-    here = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, left(a), here, 0, 0, 0);
-    next = __builtin_amdgcn_mfma_f32_16x16x4f32(1.0f, over + left(b), next, 0, 0, 0);
+// Sums along the diagonals of a 16 x 16 tile S^T (lane (r16, g): query r16, keys 4 g + e): lane (r16, g) adds
+// what its group has at distance (the tile's first key less its first query) + 4 g - r16 to `here`, and
+// at 16 more to `next`. Key e of lane r16 is on the diagonal of key 0 of the lane e to the left, or 16 on
+// where that leaves the 16 lanes.
+__device__ __forceinline__ void diagonal_sums(floatx4 s, float& here, float& next) {
+    here += s[0];
+    here += dpp_move<0x101>(s[1]);
+    here += dpp_move<0x102>(s[2]);
+    here += dpp_move<0x103>(s[3]);
+    next += dpp_move<0x11F>(s[1]);
+    next += dpp_move<0x11E>(s[2]);
+    next += dpp_move<0x11D>(s[3]);
 }
 
 // ---- dQ of 16 NW queries of a head --------------------------------------------------------------
@@ -135,7 +132,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     // (stages: as in the forward pass, arrays of their own)
     __shared__ __attribute__((aligned(16))) char stage0[KS * DQ_STAGE], stage1[KS * DQ_STAGE];
     extern __shared__ __attribute__((aligned(16))) float tab0[];
-    constexpr int QB = 16 * NW, LOADS = 16 / NW;
+    constexpr int QB = 16 * NW, LOADS = 16 / NW, HG = hist_groups(NW);
     const Quotient ht = divide(xcd_task(blockIdx.x, gridDim.x), p.by_tiles);
     const int h = ht.q, tile = ht.r, q0 = QB * tile, kvh = divide(h, p.by_each).q;
     const int tid = threadIdx.x, l = tid & 63, r16 = l & 15, g = l >> 4;
@@ -143,7 +140,8 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     const int j4 = r16 >> 2, q4 = r16 & 3;
     const int dists = 2 * p.reach + 1;
     float* const hist0 = tab0 + p.row;
-    float* const hist = hist0 + wk * dists;
+    const int pitch = hist_pitch(p.reach);
+    float* const hist = hist0 + (wk * HG + (HG == 4 ? g : 0)) * pitch;  // the lane's row of distances
 
     // The keys of the block's rows (lane l: row q0 + l), then the lane's own row.
     KeyRange tr{0, 0};
@@ -183,7 +181,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     if (has(0)) stage(kg, stage0 + kg * DQ_STAGE);
     if (BIAS == BIAS_TABLE) {
         load_bias(p, h, 1, tab0, 64 * NW * KS);
-        for (int i = l; i < dists; i += 64) hist[i] = 0.0f;
+        for (int i = tid; i < NW * KS * HG * pitch; i += 64 * NW * KS) hist0[i] = 0.0f;
     }
 
     // The row's constants.
@@ -243,8 +241,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
         const char* st = (ST ? stage1 : stage0) + kg * DQ_STAGE;
         if (has(s + 1)) stage(kg + KS * (s + 1), (ST ? stage0 : stage1) + kg * DQ_STAGE);
         if (!has(s) || kb0 + 64 <= wlo || kb0 >= whi) return;
-        floatx4 diag[3];  // sums along diagonals; those that run from one half's keys into the next's go on
-        if (BIAS == BIAS_TABLE) diag[0] = diag[1] = diag[2] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        float diag[3] = {0.0f, 0.0f, 0.0f};  // sums along diagonals; those that run into the next half's keys go on
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {  // 32 keys: kb + 16 t + 4 g + e
             const int kb = kb0 + 32 * hf;
@@ -299,22 +296,42 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
                     for (int t = 0; t < 2; t++) diagonal_sums(ds[t], diag[t], diag[t + 1]);
                 }
                 if (!far || hf == 1) {
-                    const int x0 = kb - wq0 - r16;
-                    const bool within = kb - wql >= -p.reach && kb + 47 - wq0 <= p.reach;
+                    const int x0 = kb - wq0 + 4 * g - r16;
+                    float* const to = hist + x0 + p.reach;
+                    const bool within = kb - wql >= -p.reach && kb + 47 + 12 - wq0 <= p.reach;
+                    if (HG == 4) {
+                        // (read, add, write: an LDS addition of f32 takes its lanes one by one)
+                        float was[3];
+                        int at[3];
 #pragma unroll
-                    for (int t = 0; t < 2 + hf; t++) {
-                        const int x = x0 + 16 * t;
-                        const float v = diag[t][0];
-                        if (within) {
-                            if (g == 0) __hip_atomic_fetch_add(hist + x + p.reach, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-                        } else if (g == 0) {
-                            if (x < -p.reach) far_left += v;
-                            else if (x > p.reach) far_right += v;
-                            else __hip_atomic_fetch_add(hist + x + p.reach, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                        for (int t = 0; t < 2 + hf; t++) {
+                            const int x = x0 + 16 * t;
+                            at[t] = within || (x >= -p.reach && x <= p.reach) ? 16 * t : dists - x0 - p.reach;  // (or the spare)
+                            was[t] = to[at[t]];
+                            if (!within) {
+                                far_left += x < -p.reach ? diag[t] : 0.0f;
+                                far_right += x > p.reach ? diag[t] : 0.0f;
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < 2 + hf; t++) to[at[t]] = was[t] + diag[t];
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < 2 + hf; t++) {
+                            const int x = x0 + 16 * t;
+                            far_left += x < -p.reach ? diag[t] : 0.0f;
+                            far_right += x > p.reach ? diag[t] : 0.0f;
+                            // one group of lanes after the other: no two lanes of an addition share a distance
+#pragma unroll
+                            for (int y = 0; y < 4; y++) {
+                                if (g == y && x >= -p.reach && x <= p.reach)
+                                    __hip_atomic_fetch_add(to + 16 * t, diag[t], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+                                __builtin_amdgcn_wave_barrier();
+                            }
                         }
                     }
                     diag[0] = diag[2];
-                    diag[1] = diag[2] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                    diag[1] = diag[2] = 0.0f;
                 }
             }
             if (CAP || !BF) {
@@ -340,9 +357,10 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
 
     if (BIAS == BIAS_TABLE) {
         far_left = wave_sum(far_left), far_right = wave_sum(far_right);
-        if (l == 0) hist[0] += far_left;
-        __builtin_amdgcn_wave_barrier();
-        if (l == 0) hist[dists - 1] += far_right;
+        if (l == 0) {
+            hist[0] += far_left;
+            hist[dists - 1] += far_right;
+        }
     }
     __syncthreads();
     if (BIAS == BIAS_TABLE) {
@@ -350,7 +368,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
         for (int i = tid; i < dists; i += 64 * NW * KS) {
             float s = hist0[i];
 #pragma unroll
-            for (int x = 1; x < NW * KS; x++) s += hist0[x * dists + i];
+            for (int x = 1; x < NW * KS * HG; x++) s += hist0[x * pitch + i];
             to[i] = s;
         }
     }
@@ -784,16 +802,15 @@ struct GradPlan {
 //   2029 rows  dQ 4x1 120, 4x2 123                         dK, dV 2x4x2 102, 2x2x4 111, 2x4x1 120
 //   2029 rows, prefix, capped, 4 key heads: dQ 4x2 115, 4x1 126;  dK, dV 1x2x4 128, 2x2x4 154, 2x4x1 286
 //   64 documents in 18752 rows: dQ 4x1 203, 4x2 264        dK, dV 2x4x1 205, 1x4x1 234, 2x4x2 241
-// (dQ's groups each need a row of distances to the table's reach in LDS.)
+// (dQ's groups need rows of distances to the table's reach in LDS.)
 GradPlan grad_plan(const AttnBias& a, int cus) {
     const long q16 = (long)(a.nq + 15) / 16 * a.heads, q32 = (long)(a.nq + 31) / 32 * a.heads, q64 = (long)(a.nq + 63) / 64 * a.heads;
     const long k16 = (long)(a.nk + 15) / 16 * a.kv_heads;
     GradPlan y{4, 1, 2, 4, 1};
-    const long hist = a.table ? 4L * (bias_row(a.reach) + 8 * (2 * a.reach + 1)) : 0;  // of eight waves
-    const bool room = 8 * DQ_STAGE + hist <= LDS_BYTES;
-    if (q16 <= cus) y.dq_nw = 1, y.dq_ks = 4;
-    else if (q32 <= cus && room) y.dq_nw = 2, y.dq_ks = 4;
-    else if (2 * q64 <= 3L * cus) y.dq_ks = 2;
+    auto room = [&](int nw, int ks) { return 2 * ks * DQ_STAGE + (a.table ? dq_lds(a.reach, nw, ks) : 0) <= LDS_BYTES; };
+    if (q16 <= cus && room(1, 4)) y.dq_nw = 1, y.dq_ks = 4;
+    else if (q32 <= cus && room(2, 4)) y.dq_nw = 2, y.dq_ks = 4;
+    else if (2 * q64 <= 3L * cus && room(4, 2)) y.dq_ks = 2;
     if (k16 <= cus) y.ng = 1, y.nw = 1, y.ks = 4;
     else if (k16 <= 2L * cus) y.ng = 1, y.nw = 2, y.ks = 4;
     else if (k16 <= 3L * cus) y.nw = 2, y.ks = 4;
@@ -833,9 +850,9 @@ template <bool BF, int BIAS, bool CAP, int NW, int KS>
 void launch_dq(BiasBack b, hipStream_t st) {
     constexpr int waves = NW * KS;
     static const bool ok = lds_limit(attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>,
-                                     std::min(4 * (bias_row(BIAS_MAX_REACH) + waves * (2 * BIAS_MAX_REACH + 1)), LDS_BYTES - 2 * KS * DQ_STAGE));
+                                     std::min(dq_lds(BIAS_MAX_REACH, NW, KS), LDS_BYTES - 2 * KS * DQ_STAGE));
     (void)ok;
-    const size_t lds = BIAS == BIAS_TABLE ? 4 * (b.p.row + waves * (2 * (size_t)b.p.reach + 1)) : 0;
+    const size_t lds = BIAS == BIAS_TABLE ? dq_lds(b.p.reach, NW, KS) : 0;
     b.p.by_tiles = Div(b.tiles);
     hipLaunchKernelGGL((attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>), dim3(b.tiles * b.p.heads), dim3(64 * waves), lds, st, b);
 }
