@@ -251,6 +251,15 @@ __device__ __forceinline__ void block_bias(const BiasParams& p, const float* tab
         }
     } else if (BIAS == BIAS_SLOPES) {
         const float x = (float)(kb + 4 * g - qpos);
+        // (keys all after or all before the wave's queries: a line, one operation a score in place of two)
+        if (N == 4 && (kb >= wql || kb + 16 * N - 1 <= wq0)) {
+            const float s = kb >= wql ? -slope : slope, b0 = s * x;
+#pragma unroll
+            for (int t = 0; t < N; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) base[t][e] = fmaf(s, (float)(16 * t + e), b0);
+            return;
+        }
 #pragma unroll
         for (int t = 0; t < N; t++)
 #pragma unroll
