@@ -23,35 +23,13 @@ namespace jh {
 constexpr int BIAS_STAGE = 16384;  // 64 keys: K, then V
 constexpr int BIAS_CHUNKS = 16;    // blocks that share a tile's keys, at most
 
-// The row's output again, key by key over the keys it sees: a masked key's V may hold infinities
-// or NaN, which a weight of 0 in the tile's product would turn into NaN for rows that do not see it.
-// One wave; lane l returns dimension l. qp: the row's query; m, total: its maximum and its sum.
-template <bool BF, int BIAS, bool CAP>
-__device__ float bias_row_again(const BiasParams& p, const f16* qp, int kvh, int qpos, KeyRange r, const float* tab,
-                                float slope, float m, float total) {
-    const int l = threadIdx.x & 63;
-    const f16 *kb = p.k + kvh * 64, *vb = p.v + kvh * 64;
-    float acc = 0.0f;
-    for (int j0 = r.lo; j0 < r.hi; j0 += 64) {
-        const int j = j0 + l;
-        float w = 0.0f, unused;
-        if (j < r.hi)
-            w = fast_exp2(score_of<CAP>(p, dot64<BF>(qp, kb + (int64_t)j * p.kv_stride),
-                                        bias_at<BIAS>(p, tab, slope, j - qpos), unused) - m);
-        const int n = min(64, r.hi - j0);
-        for (int x = 0; x < n; x++)
-            acc = fmaf(__shfl(w, x), widen<BF>(vb[(int64_t)(j0 + x) * p.kv_stride + l]), acc);
-    }
-    return total > 0.0f || total != total ? acc / total : 0.0f;
-}
-
 template <bool BF, int BIAS, bool CAP, int NW, int KS>
-__global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
+__global__ __launch_bounds__(64 * NW * KS, NW == 4 && !CAP ? 4 : 1) void attn_bias_kernel(BiasParams p) {
     // The two stages are arrays of their own, so that the compiler can tell a copy into one from the reads
     // of the other: in one array every LDS read waits for every copy in flight.
     __shared__ __attribute__((aligned(16))) char stage0[KS * BIAS_STAGE], stage1[KS * BIAS_STAGE];
     extern __shared__ __attribute__((aligned(16))) float tab0[];
-    __shared__ uint32_t s_last;
+    __shared__ uint32_t s_last, s_bad;
     constexpr int QB = 16 * NW, LOADS = 16 / NW;
     const int rows = p.nq * p.each;
     const Quotient ct = divide(xcd_task(blockIdx.x, gridDim.x), p.by_chunks), ht = divide(ct.q, p.by_tiles);
@@ -114,17 +92,16 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
     // exp2(fma(score, mul, -(max mul))) scales all weights by two to the rounding of max mul, which the
     // sum takes off again: nothing while |max mul| is up to 2^20. Past that (every key of a row has a
     // bias like the type's lowest value) `big` blocks subtract first.
-    float top = -INFINITY, mx = -INFINITY, neg = 0.0f, sum = 0.0f;
-    bool big = false;
+    float top, mx, neg, sum;
+    bool big;
     floatx4 o[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) o[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
     float left = 0.0f, right = 0.0f;  // a table's ends
     const int nsteps = (nblk + KS - 1) / KS;
     auto has = [&](int b) { return kg + KS * b < nblk; };
-    auto step = [&](int b, auto st_) {
+    auto step = [&](int b, auto st_, auto careful_) __attribute__((always_inline)) {
         constexpr int ST = decltype(st_)::value;
+        constexpr bool careful = decltype(careful_)::value;  // (the second time over the keys)
         stage_barrier<0>();
         const int kb = k0 + 64 * (c0 + kg + KS * b);
         const bool act = has(b) && !(kb + 64 <= wlo || kb >= whi);
@@ -133,6 +110,10 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
         if (!act) return;
         floatx4 sc[4], base[4];  // (base: the scores' initial values; with a cap, what is added after it)
         half4 vlo[2][4], vhi[2][4];
+        auto columns = [&](int hf, int dt) {
+            vlo[hf][dt] = lds_read_tr16(st + voff[dt] + 4096 * hf);
+            vhi[hf][dt] = lds_read_tr16(st + voff[dt] + 4096 * hf + 2048);
+        };
         {
             block_bias<BIAS>(p, tab, left, right, slope, kb, g, qpos, wq0, wql, base);
             half8 kf[4][2];
@@ -151,10 +132,8 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
 #pragma unroll
             for (int hf = 0; hf < 2; hf++)
 #pragma unroll
-                for (int dt = 0; dt < 4; dt++) {
-                    vlo[hf][dt] = lds_read_tr16(st + voff[dt] + 4096 * hf);
-                    vhi[hf][dt] = lds_read_tr16(st + voff[dt] + 4096 * hf + 2048);
-                }
+                for (int dt = 0; dt < 4; dt++)
+                    if (!careful) columns(hf, dt);
         }
         if (CAP) cap_scores<4, false>(p, sc, base, 1.0f);
         if (!(kb >= flo && kb + 64 <= fhi)) {
@@ -205,28 +184,43 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
                 rs += sc[t][e];
             }
         sum += rs;
+        const bool by_pair = careful && !(kb >= flo && kb + 64 <= fhi);
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
             const half8 pf = pack8<BF>(sc[2 * hf], sc[2 * hf + 1]);
+            const uintx4 pairs = by_pair ? seen_pairs([&](int c) { return (uint32_t)(kb + 32 * hf + c - kr.lo) < kspan; }) : uintx4{};
 #pragma unroll
             for (int dt = 0; dt < 4; dt++) {
+                if (careful) columns(hf, dt);
                 const half4 lo = vlo[hf][dt], hi = vhi[hf][dt];
                 const half8 vf = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                o[dt] = mma<BF>(vf, pf, o[dt]);
+                o[dt] = by_pair ? careful_mma<BF, false>(vf, pf, pairs, o[dt]) : mma<BF>(vf, pf, o[dt]);
             }
         }
     };
-    // (the first copy goes out ahead of the table's two dependent loads)
-    if (has(0)) stage(kg, stage0 + kg * BIAS_STAGE);
-    if (BIAS == BIAS_TABLE) {
-        load_bias(p, kvh * p.each, p.each, tab0, 64 * NW * KS);
-        __syncthreads();
-        left = tab[-p.reach], right = tab[p.reach];
-    }
-    for (int b = 0; b < nsteps; b += 2) {
-        step(b, std::integral_constant<int, 0>{});
-        if (b + 1 < nsteps) step(b + 1, std::integral_constant<int, 1>{});
-    }
+    if (tid == 0) s_bad = 0;
+    auto all_keys = [&](auto careful) __attribute__((always_inline)) {
+        top = mx = -INFINITY, neg = sum = 0.0f, big = false;
+#pragma unroll
+        for (int t = 0; t < 4; t++) o[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        // (the first copy goes out ahead of the table's two dependent loads)
+        if (has(0)) stage(kg, stage0 + kg * BIAS_STAGE);
+        if (BIAS == BIAS_TABLE && !careful) {
+            load_bias(p, kvh * p.each, p.each, tab0, 64 * NW * KS);
+            __syncthreads();
+            left = tab[-p.reach], right = tab[p.reach];
+        }
+        for (int b = 0; b < nsteps; b += 2) {
+            step(b, std::integral_constant<int, 0>{}, careful);
+            if (b + 1 < nsteps) step(b + 1, std::integral_constant<int, 1>{}, careful);
+        }
+    };
+    all_keys(std::false_type{});
+    // Sums that are not finite: a V that a row does not see may have made them so. Again, with the blocks
+    // that have masked pairs pair by pair (code of its own: as a branch of the first loop it cost that 15 %).
+    if (!(finite4(o[0]) && finite4(o[1]) && finite4(o[2]) && finite4(o[3])) && row < rows) s_bad = 1;
+    __syncthreads();
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(s_bad), 0)) all_keys(std::true_type{});
 
     // The key groups' maxima, sums and outputs, through LDS to group 0, in group order.
     auto merge = [&](float mk, float sk, const floatx4 (&ok)[4]) {
@@ -313,32 +307,13 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_kernel(BiasParams p) {
 
     const float total = sum_xor32(sum_xor16(sum));
     const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-    bool bad = false;
-#pragma unroll
-    for (int dt = 0; dt < 4; dt++) {
-        o[dt] = o[dt] * inv;
-#pragma unroll
-        for (int e = 0; e < 4; e++) bad |= !(fabsf(o[dt][e]) < INFINITY);
-    }
-    uint64_t again = rows_where(bad && row < rows);
-    const bool redo = (again >> r16) & 1;
-    if (row < rows && !redo) {
+    if (row < rows) {
         f16* op = p.o + (int64_t)qi * p.o_stride + h * 64 + 4 * g;
 #pragma unroll
-        for (int dt = 0; dt < 4; dt++) *(half4*)(op + 16 * dt) = pack4<BF>(o[dt]);
-    }
-    if (row < rows && p.lse && g == 0)
-        p.lse[(size_t)h * p.nq + qi] = total > 0.0f || total != total ? (mx + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -INFINITY;
-    // (wave-uniform: the rows of `again`, one after the other)
-    while (again) {
-        const int x = __builtin_ctzll(again);
-        again &= again - 1;
-        const Quotient r = divide(r0 + 16 * w + x, p.by_each);
-        const int i = r.q, y = r.r, hx = kvh * p.each + y;
-        const float s1 = BIAS == BIAS_SLOPES ? p.slopes[hx] * p.unit : 0.0f;
-        const float v = bias_row_again<BF, BIAS, CAP>(p, p.q + (int64_t)i * p.q_stride + hx * 64, kvh, p.q_first + i,
-                                                      key_range(p, i), tab0 + y * p.row, s1, __shfl(mx, x), __shfl(total, x));
-        p.o[(int64_t)i * p.o_stride + hx * 64 + l] = pack2<BF>(v, v)[0];
+        for (int dt = 0; dt < 4; dt++) *(half4*)(op + 16 * dt) = pack4<BF>(o[dt] * inv);
+        if (p.lse && g == 0)
+            p.lse[(size_t)h * p.nq + qi] =
+                total > 0.0f || total != total ? (mx + __builtin_amdgcn_logf(total)) * 0.69314718055994531f : -INFINITY;
     }
 }
 

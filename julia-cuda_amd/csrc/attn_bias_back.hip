@@ -15,7 +15,7 @@
 // - f16: dS is scaled by a power of two from |dO| (a query's own for dQ, the largest of the queries
 //   that see a block for dK and dV), so that |dO| becomes 2^3 to 2^4 and dS keeps the type's
 //   precision whatever the loss's scale: a weight of 2^-14 times a |v| of 1 is still a normal value. It
-//   overflows where a weight near 1 meets |v| > 2^11; such a row is computed again, in 32 bits (below).
+//   overflows where a weight near 1 meets |v| > 2^11; such a block is computed again at 2^-11 of it.
 // - KS key groups (or groups of queries) of NW waves share a block, each with its own stages, where
 //   the grid is small; their sums join in LDS in order.
 // - The bias's gradient in 32 bits, before dS is rounded: a 64-key block past `reach` on one side adds
@@ -23,8 +23,8 @@
 //   lane's four keys of a 16-key tile against its neighbours' queries) and added to rows of distances
 //   in LDS that no other lane group adds to (64 documents in 18752 rows: dQ alone 61 us; with the sums
 //   on masked additions 128, the groups joined by shifts and an MFMA with ones 110, so 104).
-// - A row whose sums are not finite is computed again key by key over the pairs that are not masked: a
-//   masked infinity or NaN times a weight of 0 is NaN in the tile's products.
+// - A block whose sums are not finite is computed again, its tiles with masked pairs pair by pair: a
+//   masked infinity or NaN times a weight of 0 is NaN in the tiles' products.
 #include <algorithm>
 #include <stdexcept>
 #include <string>
@@ -72,20 +72,6 @@ __device__ __forceinline__ float grad_scale(float sq) {
     int e;
     frexpf(sqrtf(sq), &e);  // < 2^e
     return ldexpf(1.0f, 4 - e);
-}
-
-// One pair's share, for the rows that go pair by pair: the weight and dA (without the scale) of query
-// i (head h) and key j. nl, dn: the row's.
-template <bool BF, int BIAS, bool CAP>
-__device__ __forceinline__ void grad_pair(const BiasBack& b, const float* tab, float slope, int h, int kvh, int i, int j,
-                                          float nl, float dn, float& w, float& da) {
-    const BiasParams& p = b.p;
-    float cap;
-    const float qk = dot64<BF>(p.q + (int64_t)i * p.q_stride + h * 64, p.k + (int64_t)j * p.kv_stride + kvh * 64);
-    const float s = score_of<CAP>(p, qk, bias_at<BIAS>(p, tab, slope, j - (p.q_first + i)), cap);
-    w = fast_exp2(s + nl);
-    const float dp = dot64<BF>(b.dout + (int64_t)i * b.do_stride + h * 64, p.v + (int64_t)j * p.kv_stride + kvh * 64);
-    da = w * (dp + dn) * cap;
 }
 
 // out[x stride] = the sum of term(x, i) over i < n, for x < m, by a block: THREADS / (m rounded up to a
@@ -138,6 +124,8 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     const int tid = threadIdx.x, l = tid & 63, r16 = l & 15, g = l >> 4;
     const int wk = __builtin_amdgcn_readfirstlane(tid >> 6), w = wk % NW, kg = wk / NW;
     const int j4 = r16 >> 2, q4 = r16 & 3;
+    __shared__ uint32_t s_bad;
+    if (tid == 0) s_bad = 0;
     const int dists = 2 * p.reach + 1;
     float* const hist0 = tab0 + p.row;
     const int pitch = hist_pitch(p.reach);
@@ -203,7 +191,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     // (past 2^20 either way: a row of biases like the type's lowest value, its weights lost in lse's rounding)
     const float nl = !real || fabsf(lse) > 1048576.0f ? -INFINITY : lse * -1.4426950408889634f;
     const float dn = real ? -d : 0.0f;
-    const float sigma = BF ? 1.0f : grad_scale(sq);
+    float sigma = BF ? 1.0f : grad_scale(sq);
     const KeyRange kr = {__shfl(tr.lo, 16 * w + r16), __shfl(tr.hi, 16 * w + r16)};
     if (kg == 0) {
         if (g == 0) {
@@ -232,10 +220,9 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     for (int dt = 0; dt < 4; dt++) toff[dt] = att_swz(4 * g + j4, 2 * dt + (q4 >> 1)) + (q4 & 1) * 8;
 
     floatx4 dq[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) dq[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto step = [&](int s, auto st_) {
+    auto step = [&](int s, auto st_, auto careful_) __attribute__((always_inline)) {
         constexpr int ST = decltype(st_)::value;
+        constexpr bool careful = decltype(careful_)::value;  // (the second time, as in the forward pass)
         stage_barrier<0>();
         const int kb0 = k0 + 64 * (kg + KS * s);
         const char* st = (ST ? stage1 : stage0) + kg * DQ_STAGE;
@@ -248,6 +235,10 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
             floatx4 base[2], sc[2], ds[2];
             half8 kf[2][2], vf[2][2];
             half4 kt[4][2];
+            auto columns = [&](int dt) {
+#pragma unroll
+                for (int y = 0; y < 2; y++) kt[dt][y] = lds_read_tr16(st + toff[dt] + 4096 * hf + 2048 * y);
+            };
             block_bias<BIAS>(p, tab, left, right, slope, kb, g, qpos, wq0, wql, base);
 #pragma unroll
             for (int t = 0; t < 2; t++)
@@ -258,8 +249,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
                 }
 #pragma unroll
             for (int dt = 0; dt < 4; dt++)
-#pragma unroll
-                for (int y = 0; y < 2; y++) kt[dt][y] = lds_read_tr16(st + toff[dt] + 4096 * hf + 2048 * y);
+                if (!careful) columns(dt);
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 sc[t] = CAP ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : base[t];
@@ -270,22 +260,18 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
                 for (int k2 = 0; k2 < 2; k2++) ds[t] = mma<BF>(vf[t][k2], gf[k2], ds[t]);
             }
             if (CAP) cap_scores<2, true>(p, sc, base, sigma);
-            if (!(kb >= flo && kb + 32 <= fhi)) {
-                const int at = kb + 4 * g - kr.lo;
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const bool ok = (uint32_t)(at + 16 * t + e) < kspan;
-                        sc[t][e] = ok ? sc[t][e] : -INFINITY;
-                        ds[t][e] = ok ? ds[t][e] : 0.0f;
-                    }
-            }
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) ds[t][e] *= fast_exp2(CAP ? sc[t][e] + nl : fmaf(sc[t][e], p.mul, nl));
-            if (BIAS == BIAS_TABLE) {
+            if (!(kb >= flo && kb + 32 <= fhi)) {  // (whatever a masked pair's score was)
+                const int at = kb + 4 * g - kr.lo;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) ds[t][e] = (uint32_t)(at + 16 * t + e) < kspan ? ds[t][e] : 0.0f;
+            }
+            if (BIAS == BIAS_TABLE && !careful) {
                 const bool far = kb - wql >= p.reach || kb + 31 - wq0 <= -p.reach;
                 if (far) {
                     const float v = ((ds[0][0] + ds[0][1]) + (ds[0][2] + ds[0][3])) + ((ds[1][0] + ds[1][1]) + (ds[1][2] + ds[1][3]));
@@ -340,19 +326,34 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
 #pragma unroll
                     for (int e = 0; e < 4; e++) ds[t][e] *= CAP ? base[t][e] : sigma;
             }
+            const bool by_pair = careful && !(kb >= flo && kb + 32 <= fhi);
+            const uintx4 pairs = by_pair ? seen_pairs([&](int c) { return (uint32_t)(kb + c - kr.lo) < kspan; }) : uintx4{};
             const half8 sf = pack8<BF>(ds[0], ds[1]);
 #pragma unroll
             for (int dt = 0; dt < 4; dt++) {
+                if (careful) columns(dt);
                 const half4 lo = kt[dt][0], hi = kt[dt][1];
                 const half8 ka = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                dq[dt] = mma<BF>(ka, sf, dq[dt]);
+                dq[dt] = by_pair ? careful_mma<BF, true>(ka, sf, pairs, dq[dt]) : mma<BF>(ka, sf, dq[dt]);
             }
         }
     };
     const int nsteps = (nblk + KS - 1) / KS;
-    for (int s = 0; s < nsteps; s += 2) {
-        step(s, std::integral_constant<int, 0>{});
-        if (s + 1 < nsteps) step(s + 1, std::integral_constant<int, 1>{});
+    auto all_keys = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) dq[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < nsteps; s += 2) {
+            step(s, std::integral_constant<int, 0>{}, careful);
+            if (s + 1 < nsteps) step(s + 1, std::integral_constant<int, 1>{}, careful);
+        }
+    };
+    all_keys(std::false_type{});
+    if (!(finite4(dq[0]) && finite4(dq[1]) && finite4(dq[2]) && finite4(dq[3])) && real) s_bad = 1;
+    __syncthreads();
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(s_bad), 0)) {
+        if (!BF) sigma *= 0x1p-11f;
+        if (has(0)) stage(kg, stage0 + kg * DQ_STAGE);
+        all_keys(std::true_type{});
     }
 
     if (BIAS == BIAS_TABLE) {
@@ -389,40 +390,16 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
     }
 
     const float back = p.scale / sigma;
-    bool bad = false;
-#pragma unroll
-    for (int dt = 0; dt < 4; dt++) {
-        dq[dt] = dq[dt] * back;
-#pragma unroll
-        for (int e = 0; e < 4; e++) bad |= !(fabsf(dq[dt][e]) < INFINITY);
-    }
-    uint64_t again = rows_where(bad && real);
-    if (real && !((again >> r16) & 1)) {
+    if (real) {
         f16* to = b.dq + (int64_t)row * b.dq_stride + h * 64 + 4 * g;
 #pragma unroll
-        for (int dt = 0; dt < 4; dt++) *(half4*)(to + 16 * dt) = pack4<BF>(dq[dt]);
-    }
-    while (again) {
-        const int y = __builtin_ctzll(again);
-        again &= again - 1;
-        const int i = q0 + 16 * w + y;
-        const KeyRange r = key_range(p, i);
-        const float inl = __shfl(nl, y), idn = __shfl(dn, y);
-        float acc = 0.0f;
-        for (int j0 = r.lo; j0 < r.hi; j0 += 64) {
-            float pw = 0.0f, da = 0.0f;
-            const int n = min(64, r.hi - j0);
-            if (l < n) grad_pair<BF, BIAS, CAP>(b, tab0, slope, h, kvh, i, j0 + l, inl, idn, pw, da);
-            for (int z = 0; z < n; z++)
-                acc = fmaf(__shfl(da, z), widen<BF>(p.k[(int64_t)(j0 + z) * p.kv_stride + kvh * 64 + l]), acc);
-        }
-        b.dq[(int64_t)i * b.dq_stride + h * 64 + l] = pack2<BF>(acc * p.scale, 0.0f)[0];
+        for (int dt = 0; dt < 4; dt++) *(half4*)(to + 16 * dt) = pack4<BF>(dq[dt] * back);
     }
 }
 
 // ---- dK and dV of 16 NG NW keys -----------------------------------------------------------------
 template <bool BF, int BIAS, bool CAP, int NG, int NW, int KS>
-__global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b) {
+__global__ __launch_bounds__(64 * NW * KS, 2) void attn_bias_dkv_kernel(BiasBack b) {
     const BiasParams& p = b.p;
     // Two stages, or three where the LDS has room: with two, a step waited for copies that it had seen
     // issued only one step before (the batch's copies and barriers alone, without the products, took
@@ -484,10 +461,8 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
     for (int x = 0; x < NG; x++)
         if (key[x] >= p.nk) kf[x][0] = kf[x][1] = vf[x][0] = vf[x][1] = half8{};
     floatx4 dk[NG][4], dv[NG][4];
-#pragma unroll
-    for (int x = 0; x < NG; x++)
-#pragma unroll
-        for (int t = 0; t < 4; t++) dk[x][t] = dv[x][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    __shared__ uint32_t s_bad;
+    if (tid == 0) s_bad = 0;
 
     uint32_t off[LOADS];
 #pragma unroll
@@ -517,191 +492,229 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
     // 64 tiles of 64 queries at a time (the bounds of 256 loaded together): those that see some of the
     // block's keys, for each query head; group kg of the block takes every KS-th.
     int4 ahead[4];
-    for (int t0 = 0; t0 < qt; t0 += 64) {
-        if ((t0 & 255) == 0) {
+    auto all_queries = [&](auto careful_) __attribute__((always_inline)) {
+        constexpr bool careful = decltype(careful_)::value;  // (the second time, as in the forward pass)
 #pragma unroll
-            for (int x = 0; x < 4; x++) ahead[x] = tile_bounds(t0 + 64 * x + l);
-        }
-        const int4 bd = ahead[0];
-        ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
-        const uint64_t seen = __builtin_amdgcn_ballot_w64(bd.x < kb + KB && bd.y > kb);
-        if (seen == 0) continue;
-        const int steps = p.each * __builtin_popcountll(seen);
-        int sub = 0;
-        uint64_t rest = seen;
-        auto skip = [&](int n) {  // (query head, tile) n further on
-            for (; n > 0; n--) {
-                rest &= rest - 1;
-                if (rest == 0) rest = seen, sub++;
+        for (int x = 0; x < NG; x++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) dk[x][t] = dv[x][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t0 = 0; t0 < qt; t0 += 64) {
+            if ((t0 & 255) == 0) {
+#pragma unroll
+                for (int x = 0; x < 4; x++) ahead[x] = tile_bounds(t0 + 64 * x + l);
             }
-        };
-        auto has = [&](int s) { return kg + KS * s < steps; };
-        struct Step {
-            int sub, t;
-        };
-        auto at_step = [&]() { return Step{sub, t0 + __builtin_ctzll(rest)}; };
-        skip(kg);
-        Step now = at_step(), then = now;  // (then: the step after, of three stages)
-        __syncthreads();  // the table; the stages of the last 64 tiles are no longer read
-        if (has(0)) stage(kvh * p.each + now.sub, now.t, stage0 + kg * DKV_STAGE);
-        if (NS == 3 && has(1)) {
-            skip(KS);
-            then = at_step();
-            stage(kvh * p.each + then.sub, then.t, stage1 + kg * DKV_STAGE);
-        }
-        if (!BF) {
-            float m = 0.0f;
-            if ((seen >> l) & 1)
-                for (int s = 0; s < p.each; s++) {
-                    const floatx4 d = *(const floatx4*)(b.max_do + (size_t)(kvh * p.each + s) * (b.nqp / 16) + 4 * (t0 + l));
-                    m = fmaxf(m, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])));
+            const int4 bd = ahead[0];
+            ahead[0] = ahead[1], ahead[1] = ahead[2], ahead[2] = ahead[3];
+            const uint64_t seen = __builtin_amdgcn_ballot_w64(bd.x < kb + KB && bd.y > kb);
+            if (seen == 0) continue;
+            const int steps = p.each * __builtin_popcountll(seen);
+            int sub = 0;
+            uint64_t rest = seen;
+            auto skip = [&](int n) {  // (query head, tile) n further on
+                for (; n > 0; n--) {
+                    rest &= rest - 1;
+                    if (rest == 0) rest = seen, sub++;
                 }
-            const float was = sigma;
-            sigma = grad_scale(max_xor32(max_xor16(row_max(m))));
-            if (sigma != was) {
-#pragma unroll
-                for (int x = 0; x < NG; x++)
-#pragma unroll
-                    for (int t = 0; t < 4; t++) dk[x][t] = dk[x][t] * (sigma / was);
-            }
-        }
-        auto step = [&](int s, auto st_) {
-            constexpr int ST = decltype(st_)::value;
-            // (all but the next step's copies have landed)
-            if (NS == 3 && has(s + 1)) stage_barrier<NS == 3 ? LOADS + 4 / NW : 0>();
-            else stage_barrier<0>();
-            if (!has(s)) return;
-            const char* st = (ST == 0 ? stage0 : ST == 1 ? stage1 : stage2) + kg * DKV_STAGE;
-            const int hx = now.sub, pos0 = p.q_first + 64 * now.t, h = kvh * p.each + hx, at_t = now.t - t0;
-            const int lo = __builtin_amdgcn_readlane(bd.x, at_t), hi = __builtin_amdgcn_readlane(bd.y, at_t);
-            const int flo = __builtin_amdgcn_readlane(bd.z, at_t), fhi = __builtin_amdgcn_readlane(bd.w, at_t);
-            const bool act = kw < hi && kw + WK > lo, full = kw >= flo && kw + WK <= fhi;
-            const float slope = BIAS == BIAS_SLOPES ? p.slopes[h] * p.unit : 0.0f;
-            const float* tab = tab0 + (BIAS == BIAS_TABLE ? hx * p.row + p.reach + BIAS_PAD : 0);
-            const float* nl = (const float*)(st + 16384);
-            const float* dn = (const float*)(st + 16384 + 256);
-            const int2* rg = (const int2*)(st + 16384 + 512);
-            now = then;
-            if (has(s + NS - 1)) {
+            };
+            auto has = [&](int s) { return kg + KS * s < steps; };
+            struct Step {
+                int sub, t;
+            };
+            auto at_step = [&]() { return Step{sub, t0 + __builtin_ctzll(rest)}; };
+            skip(kg);
+            Step now = at_step(), then = now;  // (then: the step after, of three stages)
+            __syncthreads();  // the table; the stages of the last 64 tiles are no longer read
+            if (has(0)) stage(kvh * p.each + now.sub, now.t, stage0 + kg * DKV_STAGE);
+            if (NS == 3 && has(1)) {
                 skip(KS);
                 then = at_step();
-                constexpr int TO = (ST + NS - 1) % NS;
-                stage(kvh * p.each + then.sub, then.t, (TO == 0 ? stage0 : TO == 1 ? stage1 : stage2) + kg * DKV_STAGE);
+                stage(kvh * p.each + then.sub, then.t, stage1 + kg * DKV_STAGE);
             }
-            if (NS == 2) now = then;
-            if (!act) return;
-#pragma unroll
-            for (int hf = 0; hf < 2; hf++) {  // 32 queries: rows 32 hf + 16 t + 4 g + e of the tile, column key[x]
-                half8 qa[2][2], ga[2][2];
-                floatx4 l4[2], d4[2], base[2 * NG], sc[2 * NG], ds[2 * NG];
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const int at = 32 * hf + 16 * t;
-#pragma unroll
-                    for (int k2 = 0; k2 < 2; k2++) {
-                        qa[t][k2] = *(const half8*)(st + aoff[k2] + 128 * at);
-                        ga[t][k2] = *(const half8*)(st + 8192 + aoff[k2] + 128 * at);
+            if (!BF) {
+                float m = 0.0f;
+                if ((seen >> l) & 1)
+                    for (int s = 0; s < p.each; s++) {
+                        const floatx4 d = *(const floatx4*)(b.max_do + (size_t)(kvh * p.each + s) * (b.nqp / 16) + 4 * (t0 + l));
+                        m = fmaxf(m, fmaxf(fmaxf(d[0], d[1]), fmaxf(d[2], d[3])));
                     }
-                    l4[t] = *(const floatx4*)(nl + at + 4 * g);
-                    d4[t] = *(const floatx4*)(dn + at + 4 * g);
-                }
-                if (BIAS == BIAS_TABLE) {
-                    // distances from kw - (pos0 + 32 hf + 31) to kw + WK - 1 - (pos0 + 32 hf)
-                    const int z = kw - pos0 - 32 * hf;
-                    if (z - 31 >= p.reach || z + WK - 1 <= -p.reach) {
-                        const float b0 = z > 0 ? tab[p.reach] : tab[-p.reach];
+                const float was = sigma;
+                sigma = grad_scale(max_xor32(max_xor16(row_max(m)))) * (careful ? 0x1p-11f : 1.0f);
+                if (sigma != was) {
 #pragma unroll
-                        for (int y = 0; y < 2 * NG; y++) base[y] = floatx4{b0, b0, b0, b0};
-                    } else {
-                        const float* from = tab + (z + r16 - 4 * g);
+                    for (int x = 0; x < NG; x++)
+#pragma unroll
+                        for (int t = 0; t < 4; t++) dk[x][t] = dk[x][t] * (sigma / was);
+                }
+            }
+            auto step = [&](int s, auto st_) __attribute__((always_inline)) {
+                constexpr int ST = decltype(st_)::value;
+                // (all but the next step's copies have landed)
+                if (NS == 3 && has(s + 1)) stage_barrier<NS == 3 ? LOADS + 4 / NW : 0>();
+                else stage_barrier<0>();
+                if (!has(s)) return;
+                const char* st = (ST == 0 ? stage0 : ST == 1 ? stage1 : stage2) + kg * DKV_STAGE;
+                const int hx = now.sub, pos0 = p.q_first + 64 * now.t, h = kvh * p.each + hx, at_t = now.t - t0;
+                const int lo = __builtin_amdgcn_readlane(bd.x, at_t), hi = __builtin_amdgcn_readlane(bd.y, at_t);
+                const int flo = __builtin_amdgcn_readlane(bd.z, at_t), fhi = __builtin_amdgcn_readlane(bd.w, at_t);
+                const bool act = kw < hi && kw + WK > lo, full = kw >= flo && kw + WK <= fhi;
+                const float slope = BIAS == BIAS_SLOPES ? p.slopes[h] * p.unit : 0.0f;
+                const float* tab = tab0 + (BIAS == BIAS_TABLE ? hx * p.row + p.reach + BIAS_PAD : 0);
+                const float* nl = (const float*)(st + 16384);
+                const float* dn = (const float*)(st + 16384 + 256);
+                const int2* rg = (const int2*)(st + 16384 + 512);
+                now = then;
+                if (has(s + NS - 1)) {
+                    skip(KS);
+                    then = at_step();
+                    constexpr int TO = (ST + NS - 1) % NS;
+                    stage(kvh * p.each + then.sub, then.t, (TO == 0 ? stage0 : TO == 1 ? stage1 : stage2) + kg * DKV_STAGE);
+                }
+                if (NS == 2) now = then;
+                if (!act) return;
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {  // 32 queries: rows 32 hf + 16 t + 4 g + e of the tile, column key[x]
+                    half8 qa[2][2], ga[2][2];
+                    floatx4 l4[2], d4[2], base[2 * NG], sc[2 * NG], ds[2 * NG];
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const int at = 32 * hf + 16 * t;
+#pragma unroll
+                        for (int k2 = 0; k2 < 2; k2++) {
+                            qa[t][k2] = *(const half8*)(st + aoff[k2] + 128 * at);
+                            ga[t][k2] = *(const half8*)(st + 8192 + aoff[k2] + 128 * at);
+                        }
+                        l4[t] = *(const floatx4*)(nl + at + 4 * g);
+                        d4[t] = *(const floatx4*)(dn + at + 4 * g);
+                    }
+                    if (BIAS == BIAS_TABLE) {
+                        // distances from kw - (pos0 + 32 hf + 31) to kw + WK - 1 - (pos0 + 32 hf)
+                        const int z = kw - pos0 - 32 * hf;
+                        if (z - 31 >= p.reach || z + WK - 1 <= -p.reach) {
+                            const float b0 = z > 0 ? tab[p.reach] : tab[-p.reach];
+#pragma unroll
+                            for (int y = 0; y < 2 * NG; y++) base[y] = floatx4{b0, b0, b0, b0};
+                        } else {
+                            const float* from = tab + (z + r16 - 4 * g);
+#pragma unroll
+                            for (int x = 0; x < NG; x++)
+#pragma unroll
+                                for (int t = 0; t < 2; t++)
+#pragma unroll
+                                    for (int e = 0; e < 4; e++) base[2 * x + t][e] = from[16 * x - 16 * t - e];
+                        }
+                    } else if (BIAS == BIAS_SLOPES) {
+                        const float y = (float)(kw + r16 - pos0 - 32 * hf - 4 * g);
 #pragma unroll
                         for (int x = 0; x < NG; x++)
 #pragma unroll
                             for (int t = 0; t < 2; t++)
 #pragma unroll
-                                for (int e = 0; e < 4; e++) base[2 * x + t][e] = from[16 * x - 16 * t - e];
+                                for (int e = 0; e < 4; e++) base[2 * x + t][e] = -slope * fabsf(y + (float)(16 * x - 16 * t - e));
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 2 * NG; y++) base[y] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
                     }
-                } else if (BIAS == BIAS_SLOPES) {
-                    const float y = (float)(kw + r16 - pos0 - 32 * hf - 4 * g);
 #pragma unroll
                     for (int x = 0; x < NG; x++)
 #pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            const int y = 2 * x + t;
+                            sc[y] = CAP ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : base[y];
+                            ds[y] = d4[t];
+#pragma unroll
+                            for (int k2 = 0; k2 < 2; k2++) sc[y] = mma<BF>(qa[t][k2], kf[x][k2], sc[y]);
+#pragma unroll
+                            for (int k2 = 0; k2 < 2; k2++) ds[y] = mma<BF>(ga[t][k2], vf[x][k2], ds[y]);
+                        }
+                    if (CAP) cap_scores<2 * NG, true>(p, sc, base, sigma);
+                    if (!full) {
+#pragma unroll
                         for (int t = 0; t < 2; t++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) base[2 * x + t][e] = -slope * fabsf(y + (float)(16 * x - 16 * t - e));
-                } else {
+                            for (int e = 0; e < 4; e++) {
+                                const int2 k = rg[32 * hf + 16 * t + 4 * g + e];
 #pragma unroll
-                    for (int y = 0; y < 2 * NG; y++) base[y] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-                }
-#pragma unroll
-                for (int x = 0; x < NG; x++)
-#pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        const int y = 2 * x + t;
-                        sc[y] = CAP ? floatx4{0.0f, 0.0f, 0.0f, 0.0f} : base[y];
-                        ds[y] = d4[t];
-#pragma unroll
-                        for (int k2 = 0; k2 < 2; k2++) sc[y] = mma<BF>(qa[t][k2], kf[x][k2], sc[y]);
-#pragma unroll
-                        for (int k2 = 0; k2 < 2; k2++) ds[y] = mma<BF>(ga[t][k2], vf[x][k2], ds[y]);
-                    }
-                if (CAP) cap_scores<2 * NG, true>(p, sc, base, sigma);
-                if (!full) {
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int2 k = rg[32 * hf + 16 * t + 4 * g + e];
-#pragma unroll
-                            for (int x = 0; x < NG; x++) {
-                                const bool ok = (uint32_t)(key[x] - k.x) < (uint32_t)k.y;
-                                sc[2 * x + t][e] = ok ? sc[2 * x + t][e] : -INFINITY;
-                                ds[2 * x + t][e] = ok ? ds[2 * x + t][e] : 0.0f;
+                                for (int x = 0; x < NG; x++) {
+                                    const bool ok = (uint32_t)(key[x] - k.x) < (uint32_t)k.y;
+                                    sc[2 * x + t][e] = ok ? sc[2 * x + t][e] : -INFINITY;
+                                    ds[2 * x + t][e] = ok ? ds[2 * x + t][e] : 0.0f;
+                                }
                             }
-                        }
-                }
-                half4 gt[4][2], qt4[4][2];
-#pragma unroll
-                for (int dt = 0; dt < 4; dt++)
-#pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        gt[dt][y] = lds_read_tr16(st + 8192 + toff[dt] + 4096 * hf + 2048 * y);
-                        qt4[dt][y] = lds_read_tr16(st + toff[dt] + 4096 * hf + 2048 * y);
                     }
-                half8 pf[NG], sf[NG];
+                    half4 gt[4][2], qt4[4][2];
+                    auto columns = [&](int dt) {
 #pragma unroll
-                for (int x = 0; x < NG; x++) {
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int y = 2 * x + t;
-                            sc[y][e] = fast_exp2(CAP ? sc[y][e] + l4[t][e] : fmaf(sc[y][e], p.mul, l4[t][e]));
-                            ds[y][e] *= sc[y][e];
-                            if (CAP || !BF) ds[y][e] *= CAP ? base[y][e] : sigma;
+                        for (int y = 0; y < 2; y++) {
+                            gt[dt][y] = lds_read_tr16(st + 8192 + toff[dt] + 4096 * hf + 2048 * y);
+                            qt4[dt][y] = lds_read_tr16(st + toff[dt] + 4096 * hf + 2048 * y);
                         }
-                    pf[x] = pack8<BF>(sc[2 * x], sc[2 * x + 1]);
-                    sf[x] = pack8<BF>(ds[2 * x], ds[2 * x + 1]);
-                }
+                    };
 #pragma unroll
-                for (int dt = 0; dt < 4; dt++) {
-                    const half8 a = {gt[dt][0][0], gt[dt][0][1], gt[dt][0][2], gt[dt][0][3], gt[dt][1][0], gt[dt][1][1], gt[dt][1][2], gt[dt][1][3]};
-                    const half8 c = {qt4[dt][0][0], qt4[dt][0][1], qt4[dt][0][2], qt4[dt][0][3], qt4[dt][1][0], qt4[dt][1][1], qt4[dt][1][2], qt4[dt][1][3]};
+                    for (int dt = 0; dt < 4; dt++)
+                        if (!careful) columns(dt);
+                    half8 pf[NG], sf[NG];
 #pragma unroll
                     for (int x = 0; x < NG; x++) {
-                        dv[x][dt] = mma<BF>(a, pf[x], dv[x][dt]);
-                        dk[x][dt] = mma<BF>(c, sf[x], dk[x][dt]);
+#pragma unroll
+                        for (int t = 0; t < 2; t++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int y = 2 * x + t;
+                                sc[y][e] = fast_exp2(CAP ? sc[y][e] + l4[t][e] : fmaf(sc[y][e], p.mul, l4[t][e]));
+                                ds[y][e] *= sc[y][e];
+                                if (CAP || !BF) ds[y][e] *= CAP ? base[y][e] : sigma;
+                            }
+                        pf[x] = pack8<BF>(sc[2 * x], sc[2 * x + 1]);
+                        sf[x] = pack8<BF>(ds[2 * x], ds[2 * x + 1]);
+                    }
+                    if (careful && !full) {
+#pragma unroll
+                        for (int x = 0; x < NG; x++) {
+                            const uintx4 pairs = seen_pairs([&](int c) {
+                                const int2 k = rg[32 * hf + c];
+                                return (uint32_t)(key[x] - k.x) < (uint32_t)k.y;
+                            });
+#pragma unroll
+                            for (int dt = 0; dt < 4; dt++) {
+                                columns(dt);
+                                const half8 a = {gt[dt][0][0], gt[dt][0][1], gt[dt][0][2], gt[dt][0][3], gt[dt][1][0], gt[dt][1][1], gt[dt][1][2], gt[dt][1][3]};
+                                const half8 c = {qt4[dt][0][0], qt4[dt][0][1], qt4[dt][0][2], qt4[dt][0][3], qt4[dt][1][0], qt4[dt][1][1], qt4[dt][1][2], qt4[dt][1][3]};
+                                dv[x][dt] = careful_mma<BF, false>(a, pf[x], pairs, dv[x][dt]);
+                                dk[x][dt] = careful_mma<BF, true>(c, sf[x], pairs, dk[x][dt]);
+                            }
+                        }
+                        continue;
+                    }
+#pragma unroll
+                    for (int dt = 0; dt < 4; dt++) {
+                        if (careful) columns(dt);
+                        const half8 a = {gt[dt][0][0], gt[dt][0][1], gt[dt][0][2], gt[dt][0][3], gt[dt][1][0], gt[dt][1][1], gt[dt][1][2], gt[dt][1][3]};
+                        const half8 c = {qt4[dt][0][0], qt4[dt][0][1], qt4[dt][0][2], qt4[dt][0][3], qt4[dt][1][0], qt4[dt][1][1], qt4[dt][1][2], qt4[dt][1][3]};
+#pragma unroll
+                        for (int x = 0; x < NG; x++) {
+                            dv[x][dt] = mma<BF>(a, pf[x], dv[x][dt]);
+                            dk[x][dt] = mma<BF>(c, sf[x], dk[x][dt]);
+                        }
                     }
                 }
+            };
+            const int nsteps = (steps + KS - 1) / KS;
+            for (int s = 0; s < nsteps; s += NS) {
+                step(s, std::integral_constant<int, 0>{});
+                if (s + 1 < nsteps) step(s + 1, std::integral_constant<int, 1>{});
+                if (NS == 3 && s + 2 < nsteps) step(s + 2, std::integral_constant<int, NS - 1>{});
             }
-        };
-        const int nsteps = (steps + KS - 1) / KS;
-        for (int s = 0; s < nsteps; s += NS) {
-            step(s, std::integral_constant<int, 0>{});
-            if (s + 1 < nsteps) step(s + 1, std::integral_constant<int, 1>{});
-            if (NS == 3 && s + 2 < nsteps) step(s + 2, std::integral_constant<int, NS - 1>{});
         }
-    }
+    };
+    all_queries(std::false_type{});
+    bool fine = true;
+#pragma unroll
+    for (int x = 0; x < NG; x++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) fine = fine && (key[x] >= p.nk || (finite4(dk[x][t]) && finite4(dv[x][t])));
+    if (!fine) s_bad = 1;
+    __syncthreads();
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(s_bad), 0)) all_queries(std::true_type{});
 
     if (KS > 1) {
         __syncthreads();
@@ -732,52 +745,12 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dkv_kernel(BiasBack b)
     const float back = p.scale / sigma;
 #pragma unroll
     for (int x = 0; x < NG; x++) {
-        bool bad = false;
+        if (key[x] >= p.nk) continue;
+        const int64_t at = (int64_t)key[x] * b.dkv_stride + kvh * 64 + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < 4; dt++) {
-            dk[x][dt] = dk[x][dt] * back;
-#pragma unroll
-            for (int e = 0; e < 4; e++) bad |= !(fabsf(dk[x][dt][e]) < INFINITY) || !(fabsf(dv[x][dt][e]) < INFINITY);
-        }
-        uint64_t again = rows_where(bad && key[x] < p.nk);
-        if (key[x] < p.nk && !((again >> r16) & 1)) {
-            const int64_t at = (int64_t)key[x] * b.dkv_stride + kvh * 64 + 4 * g;
-#pragma unroll
-            for (int dt = 0; dt < 4; dt++) {
-                *(half4*)(b.dk + at + 16 * dt) = pack4<BF>(dk[x][dt]);
-                *(half4*)(b.dv + at + 16 * dt) = pack4<BF>(dv[x][dt]);
-            }
-        }
-        while (again) {
-            const int y = __builtin_ctzll(again);
-            again &= again - 1;
-            const int j = kw + 16 * x + y;
-            float ak = 0.0f, av = 0.0f;
-            for (int sub = 0; sub < p.each; sub++) {
-                const int h = kvh * p.each + sub;
-                const float slope = BIAS == BIAS_SLOPES ? p.slopes[h] * p.unit : 0.0f;
-                for (int i0 = 0; i0 < p.nq; i0 += 64) {
-                    const int i = i0 + l;
-                    float pw = 0.0f, da = 0.0f;
-                    bool ok = false;
-                    if (i < p.nq) {
-                        const float* of = row_info(b, h, i);
-                        const int2 r = *(const int2*)(of + 128 + (i & 63));
-                        ok = (uint32_t)(j - r.x) < (uint32_t)r.y;
-                        if (ok) grad_pair<BF, BIAS, CAP>(b, tab0 + sub * p.row, slope, h, kvh, i, j, of[0], of[64], pw, da);
-                    }
-                    uint64_t some = __builtin_amdgcn_ballot_w64(ok);
-                    while (some) {
-                        const int z = __builtin_ctzll(some);
-                        some &= some - 1;
-                        av = fmaf(__shfl(pw, z), widen<BF>(b.dout[(int64_t)(i0 + z) * b.do_stride + h * 64 + l]), av);
-                        ak = fmaf(__shfl(da, z), widen<BF>(p.q[(int64_t)(i0 + z) * p.q_stride + h * 64 + l]), ak);
-                    }
-                }
-            }
-            const int64_t at = (int64_t)j * b.dkv_stride + kvh * 64 + l;
-            b.dk[at] = pack2<BF>(ak * p.scale, 0.0f)[0];
-            b.dv[at] = pack2<BF>(av, 0.0f)[0];
+            *(half4*)(b.dk + at + 16 * dt) = pack4<BF>(dk[x][dt] * back);
+            *(half4*)(b.dv + at + 16 * dt) = pack4<BF>(dv[x][dt]);
         }
     }
 }
@@ -787,7 +760,7 @@ namespace {
 
 [[noreturn]] void fail(const std::string& m) { throw std::runtime_error("attention_bias_backward: " + m); }
 
-constexpr int LDS_BYTES = 160 * 1024;
+constexpr int LDS_BYTES = 160 * 1024 - 64;  // (the rest: a flag)
 
 // The tiles of a call: 16 dq_nw queries, 16 ng nw keys a block, in ks groups.
 struct GradPlan {

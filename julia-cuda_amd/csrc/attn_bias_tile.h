@@ -161,18 +161,6 @@ __device__ __forceinline__ void load_bias(const BiasParams& p, int head, int n, 
     }
 }
 
-// A row of f16 / bf16 (64 values) times another, for the paths that go key by key.
-template <bool BF>
-__device__ __forceinline__ float dot64(const f16* a, const f16* b) {
-    float s = 0.0f;
-    for (int c = 0; c < 64; c += 8) {
-        const half8 x = *(const half8*)(a + c), y = *(const half8*)(b + c);
-#pragma unroll
-        for (int e = 0; e < 8; e++) s = fmaf(widen<BF>(x[e]), widen<BF>(y[e]), s);
-    }
-    return s;
-}
-
 // N x 4 capped scores in place from q . k, base in them; slope: the tanh's slope times `by`, into base.
 // Whether every one of the wave's is small is asked first: those of a model usually are, and the
 // polynomial takes 7 operations where the other takes 11 (an exponential and a reciprocal at four each).
@@ -209,27 +197,6 @@ __device__ __forceinline__ void cap_scores(const BiasParams& p, floatx4 (&sc)[N]
                 if (SLOPE) base[t][e] = (4.0f * by) * fmaf(-r, r, r);
             }
     }
-}
-
-// A score's weight in the exp2 domain (before the row's log-sum is taken off) from q . k, the
-// tanh's slope in `slope` (1 without a cap). base: the bias in the scores' units.
-template <bool CAP>
-__device__ __forceinline__ float score_of(const BiasParams& p, float qk, float base, float& slope) {
-    if (CAP) {
-        const float r = __builtin_amdgcn_rcpf(fast_exp2(qk * p.pre) + 1.0f);
-        slope = 4.0f * fmaf(-r, r, r);
-        return fmaf(-2.0f * p.off, r, base + p.off);
-    }
-    slope = 1.0f;
-    return (qk + base) * p.mul;
-}
-
-// The bias of head h (tab: its row in LDS) at distance t, in the same units.
-template <int BIAS>
-__device__ __forceinline__ float bias_at(const BiasParams& p, const float* tab, float slope, int t) {
-    if (BIAS == BIAS_TABLE) return tab[min(max(t, -p.reach), p.reach) + p.reach + BIAS_PAD];
-    if (BIAS == BIAS_SLOPES) return -slope * fabsf((float)t);
-    return 0.0f;
 }
 
 // The biases of 16 N keys from kb on for a lane's query (S^T: keys kb + 16 t + 4 g + e): tab, the lane's
@@ -282,11 +249,55 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// Which of a wave's 16 rows (one a lane % 16) have a lane where `bad` holds.
-__device__ __forceinline__ uint64_t rows_where(bool bad) {
-    uint64_t b = __builtin_amdgcn_ballot_w64(bad);
-    b = (b | b >> 32) & 0xffffffffull;
-    return (b | b >> 16) & 0xffffull;
+// The pairs of a product's 32 rows (16 (i / 4) + 4 (lane / 16) + i % 4, as pack8 lays them) that exist: 16 bits
+// each, all set where seen(row) holds.
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+template <typename F>
+__device__ __forceinline__ uintx4 seen_pairs(F&& seen) {
+    const int g = (threadIdx.x & 63) >> 4;
+    uintx4 m;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int c = 16 * (i >> 1) + 4 * g + 2 * (i & 1);
+        m[i] = (seen(c) ? 0xffffu : 0u) | (seen(c + 1) ? 0xffff0000u : 0u);
+    }
+    return m;
+}
+// acc += a . w where a masked pair's value may be infinite or NaN (times a weight of 0 it would make the sum
+// NaN): the finite values' product, and a second one that counts each sum's infinities of either sign, NaN
+// as one of both. ANY: an infinity makes the sum NaN (its own weight is a difference that it made NaN). Only a
+// block whose sums were not finite comes here.
+template <bool BF, bool ANY>
+__device__ __forceinline__ floatx4 careful_mma(half8 a, half8 w, uintx4 pairs, floatx4 acc) {
+    constexpr uint32_t E = BF ? 0x7f80 : 0x7c00, ONE = BF ? 0x3f80 : 0x3c00, C64 = BF ? 0x4280 : 0x5400, C65 = BF ? 0x4282 : 0x5410;
+    const uintx4 av = __builtin_bit_cast(uintx4, a), wv = __builtin_bit_cast(uintx4, w);
+    uintx4 value, flag;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t v = 0, f = 0;
+#pragma unroll
+        for (int y = 0; y < 32; y += 16) {
+            const uint32_t u = (av[i] >> y) & 0xffff;
+            const uint32_t sort = ANY || (u & 0x7fff) > E ? C65 : u >> 15 ? C64 : ONE;
+            v |= ((u & E) == E ? 0 : u) << y;
+            f |= ((u & E) == E ? sort : 0) << y;
+        }
+        value[i] = v, flag[i] = f;
+    }
+    acc = mma<BF>(__builtin_bit_cast(half8, value), __builtin_bit_cast(half8, wv & pairs), acc);
+    const floatx4 n = mma<BF>(__builtin_bit_cast(half8, flag), __builtin_bit_cast(half8, pairs & (ONE * 0x10001u)),
+                              floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+    for (int e = 0; e < 4; e++) {  // (32 rows at most of each sort: exact)
+        const float neg = floorf(n[e] * 0.015625f);
+        acc[e] += n[e] > 64.0f * neg ? INFINITY : 0.0f;
+        acc[e] += neg > 0.0f ? -INFINITY : 0.0f;
+    }
+    __builtin_amdgcn_sched_barrier(0);  // (one product after the other: registers)
+    return acc;
+}
+__device__ __forceinline__ bool finite4(floatx4 v) {
+    return fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY;
 }
 
 }  // namespace jh

@@ -249,6 +249,62 @@ def test_masked_infinities_and_nan_stay_where_they_are(torch_cuda, R, type):
     assert not bool(torch.isfinite(A.o[70:130, 64:]).all(1).any())
 
 
+@pytest.mark.parametrize("type,bias,cap,n,window", [("f16", "table", 0.0, 700, 40), ("bf16", "slopes", 20.0, 700, 0),
+                                                    ("f16", "none", 0.0, 2500, 150), ("bf16", "table", 5.0, 2500, 0)])
+def test_nan_in_one_key_reaches_the_rows_that_see_it_alone(torch_cuda, R, type, bias, cap, n, window):
+    """A NaN in a key and an infinity in a value of a causal document, in every tile layout of the launches:
+    rows that see neither keep the formula's results, the others are not finite where those are not."""
+    torch = torch_cuda
+    say("one key", type, bias, cap, n, window)
+    A = Attention(torch, R, type, n, heads=2, bias=bias, cap=cap, window=window, lens=[n], prefix=[0], seed=21)
+    at = n // 2 + 5
+    A.qkv[at, 64 * 2: 64 * 4] = math.nan  # k of both heads
+    A.qkv[at + 2, 64 * 4 + 7] = math.inf  # one column of the first head's v
+    A.forward()
+    A.backward()
+    clean = Attention(torch, R, type, n, heads=2, bias=bias, cap=cap, window=window, lens=[n], prefix=[0], seed=21)
+    clean.qkv[at: at + 3] = 0  # (what its rows that see neither key read is the same)
+    ref = clean.reference(True)
+    bound = R.attention_bounds(ref, type, cap)
+    i = torch.arange(n)
+    sees = (i >= at) & ((i - at - 2 <= window) if window else i >= 0)
+    o, dq, dk, dv = (x.cpu() for x in (A.o[:n].reshape(-1, 2, 64), *A.parts(A.dqkv)))
+    assert R.worst(o[~sees], ref["o"][~sees], bound["o"][~sees]) <= 1.0
+    assert R.worst(dq[~sees], ref["dq"][~sees], bound["dq"][~sees]) <= 1.0
+    sees_k = (i >= at) & ((i - at <= window) if window else i >= 0)
+    assert bool(torch.isnan(o[sees_k]).all()) and bool(torch.isnan(dq[sees_k]).all())
+    # keys that no row with a NaN sees: those behind every such row
+    if window:
+        far = (i > at + 3 + 2 * window) | (i < at - window)
+        assert int(far.sum()) > 0
+        assert bool(torch.isfinite(dk[far]).all()) and bool(torch.isfinite(dv[far]).all())
+        assert R.worst(dk[far], ref["dk"][far], bound["dk"][far]) <= 1.0
+        assert R.worst(dv[far], ref["dv"][far], bound["dv"][far]) <= 1.0
+
+
+def test_nan_everywhere_costs_two_passes(torch_cuda, R):
+    """Values, keys and gradients of NaN in 6000 rows: every result is NaN, in twice an ordinary call's time
+    at most (held to 20 of them: a pass for every row would be hundreds)."""
+    torch = torch_cuda
+    A = Attention(torch, R, "f16", 6000, heads=4, bias="table", lens=[6000], prefix=[0], seed=22)
+
+    def ms():
+        A.forward(), A.backward()
+        t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        t[0].record()
+        A.forward(), A.backward()
+        t[1].record()
+        torch.cuda.synchronize()
+        return t[0].elapsed_time(t[1])
+
+    plain = ms()
+    A.qkv[:, 2 * 64 * 4:] = math.nan
+    A.dout[:] = math.nan
+    say("NaN everywhere")
+    assert ms() <= 20 * max(plain, 0.5)
+    assert bool(torch.isnan(A.o[:6000]).all()) and all(bool(torch.isnan(x).all()) for x in A.parts(A.dqkv))
+
+
 def test_biases_of_the_lowest_value(torch_cuda, R):
     """A bucket of the lowest f32 leaves its keys no weight; where every key has it, all have the same,
     and -inf in every key is a row that sees none."""
