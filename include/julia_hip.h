@@ -209,7 +209,8 @@ enum { JULIA_HIP_F16 = 0, JULIA_HIP_BF16 = 1, JULIA_HIP_F32 = 2 };
  * does not see have no effect on it, whatever they hold.
  * Strides are in elements between rows, multiples of 8 up to 2^22 and at least a row's width; q, k, v,
  * o are 16-byte aligned (rows of a packed qkv do). kv_heads divides heads: query head h reads
- * key head h / (heads / kv_heads). Scores, weights and sums are f32; weights are rounded to the
+ * key head h / (heads / kv_heads). nq heads and nk kv_heads are up to 2^30. What a call writes, here and
+ * for the gradients, overlaps none of what it reads nor its other results. Scores, weights and sums are f32; weights are rounded to the
  * type for the product with v. */
 typedef struct {
     int type; /* JULIA_HIP_F16 or JULIA_HIP_BF16 */
@@ -255,11 +256,11 @@ int julia_hip_attention_bias_backward(const julia_hip_attention_bias_args *a,
 
 /* y = (x - mean) / sqrt(var + eps) . gamma + beta over rows of d values (1 to 8192) in `type`, any
  * row stride from d on; gamma, beta (nullable) and stats ([rows][2], mean and 1 / sqrt(var + eps),
- * nullable) f32. y may be x. */
+ * nullable) f32. y may be x, at x's stride; nothing else that a call writes overlaps what it reads. */
 int julia_hip_layer_norm(int type, const void *x, int64_t x_stride, int rows, int d,
                          const float *gamma, const float *beta, float eps, void *y,
                          int64_t y_stride, float *stats, void *stream, char *err, size_t err_len);
-/* Its gradients: dx in `type` (may be dy or x), dgamma and dbeta (nullable) [d] f32, summed over the
+/* Its gradients: dx in `type` (may be dy or x, at its stride), dgamma and dbeta (nullable) [d] f32, summed over the
  * rows in a fixed order; all written, not added to. The scratch: julia_hip_layer_norm_scratch. */
 int julia_hip_layer_norm_backward(int type, const void *x, int64_t x_stride, const void *dy,
                                   int64_t dy_stride, int rows, int d, const float *gamma,

@@ -10,9 +10,15 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "kernels.h"
 
 namespace jh {
+
+// Lets a kernel have `bytes` of dynamic LDS on the current device, asked for once a device (`devices`: a
+// bit each, the kernel's own).
+bool dynamic_lds(std::atomic<uint64_t>& devices, const void* kernel, int bytes);
 
 enum { BIAS_NONE = 0, BIAS_TABLE = 1, BIAS_SLOPES = 2 };
 

@@ -333,12 +333,23 @@ void check_rows(const char* what, const void* p, int64_t stride, int width) {
 
 }  // namespace
 
+bool dynamic_lds(std::atomic<uint64_t>& devices, const void* kernel, int bytes) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return false;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (devices.load(std::memory_order_relaxed) & bit) return true;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+    devices.fetch_or(bit, std::memory_order_relaxed);
+    return true;
+}
+
 void attn_bias_check(const AttnBias& a, const AttnBiasGrads* g) {
     if (a.nq < 0 || a.nk < 0 || a.nq > (1 << 24) || a.nk >= (1 << 30)) fail("a bad number of queries or keys");
     if (a.heads < 1 || a.heads > 256 || a.kv_heads < 1 || a.heads % a.kv_heads)
         fail(std::to_string(a.heads) + " heads cannot share " + std::to_string(a.kv_heads) + " key heads (up to 256 heads)");
     const int each = a.heads / a.kv_heads;
     if ((int64_t)a.nq * a.heads > (1 << 30)) fail("more than 2^30 rows of heads");
+    if ((int64_t)a.nk * a.kv_heads > (1 << 30)) fail("more than 2^30 keys of heads");
     if (a.q_first < 0 || a.q_first >= (1 << 30)) fail("q_first must be from 0 to 2^30");
     if (!(a.scale >= 1e-6f && a.scale <= 1e6f)) fail("the scale must be from 1e-6 to 1e6");
     if (!(a.cap == 0.0f || (a.cap >= 1e-3f && a.cap <= 1e6f))) fail("the cap must be 0 or from 1e-3 to 1e6");
@@ -431,10 +442,9 @@ BiasPlan bias_plan(const AttnBias& a, int cus) {
 
 template <bool BF, int BIAS, bool CAP, int NW, int KS>
 void launch_tile(const BiasParams& p, long tiles, hipStream_t st) {
-    static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(attn_bias_kernel<BF, BIAS, CAP, NW, KS>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               4 * BIAS_MAX_TABLE) == hipSuccess;
-    if (!ok) fail("the kernel cannot have its LDS");
+    static std::atomic<uint64_t> devices{0};
+    if (!dynamic_lds(devices, reinterpret_cast<const void*>(attn_bias_kernel<BF, BIAS, CAP, NW, KS>), 4 * BIAS_MAX_TABLE))
+        fail("the kernel cannot have its LDS");
     const size_t lds = BIAS == BIAS_TABLE ? 4 * (size_t)p.each * p.row : 0;
     hipLaunchKernelGGL((attn_bias_kernel<BF, BIAS, CAP, NW, KS>), dim3((unsigned)(tiles * p.chunks)), dim3(64 * NW * KS), lds, st, p);
 }

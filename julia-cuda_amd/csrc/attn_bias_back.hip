@@ -399,7 +399,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
 
 // ---- dK and dV of 16 NG NW keys -----------------------------------------------------------------
 template <bool BF, int BIAS, bool CAP, int NG, int NW, int KS>
-__global__ __launch_bounds__(64 * NW * KS, 2) void attn_bias_dkv_kernel(BiasBack b) {
+__global__ __launch_bounds__(64 * NW * KS, KS == 1 ? 2 : 1) void attn_bias_dkv_kernel(BiasBack b) {
     const BiasParams& p = b.p;
     // Two stages, or three where the LDS has room: with two, a step waited for copies that it had seen
     // issued only one step before (the batch's copies and barriers alone, without the products, took
@@ -812,19 +812,13 @@ Layout layout(const AttnBias& a, const GradPlan& plan) {
     return y;
 }
 
-template <typename K>
-bool lds_limit(K kernel, int bytes) {
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
-        fail("a kernel cannot have its LDS");
-    return true;
-}
-
 template <bool BF, int BIAS, bool CAP, int NW, int KS>
 void launch_dq(BiasBack b, hipStream_t st) {
     constexpr int waves = NW * KS;
-    static const bool ok = lds_limit(attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>,
-                                     std::min(dq_lds(BIAS_MAX_REACH, NW, KS), LDS_BYTES - 2 * KS * DQ_STAGE));
-    (void)ok;
+    static std::atomic<uint64_t> devices{0};
+    if (!dynamic_lds(devices, reinterpret_cast<const void*>(attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>),
+                     std::min(dq_lds(BIAS_MAX_REACH, NW, KS), LDS_BYTES - 2 * KS * DQ_STAGE)))
+        fail("a kernel cannot have its LDS");
     const size_t lds = BIAS == BIAS_TABLE ? dq_lds(b.p.reach, NW, KS) : 0;
     b.p.by_tiles = Div(b.tiles);
     hipLaunchKernelGGL((attn_bias_dq_kernel<BF, BIAS, CAP, NW, KS>), dim3(b.tiles * b.p.heads), dim3(64 * waves), lds, st, b);
@@ -832,8 +826,9 @@ void launch_dq(BiasBack b, hipStream_t st) {
 
 template <bool BF, int BIAS, bool CAP, int NG, int NW, int KS>
 void launch_dkv(BiasBack b, hipStream_t st) {
-    static const bool ok = lds_limit(attn_bias_dkv_kernel<BF, BIAS, CAP, NG, NW, KS>, 4 * BIAS_MAX_TABLE);
-    (void)ok;
+    static std::atomic<uint64_t> devices{0};
+    if (!dynamic_lds(devices, reinterpret_cast<const void*>(attn_bias_dkv_kernel<BF, BIAS, CAP, NG, NW, KS>), 4 * BIAS_MAX_TABLE))
+        fail("a kernel cannot have its LDS");
     const int tiles = (b.p.nk + 16 * NG * NW - 1) / (16 * NG * NW);
     b.dkv_blocks = tiles * b.p.kv_heads, b.p.by_tiles = Div(std::max(tiles, 1));
     const int blocks = b.dkv_blocks + (BIAS == BIAS_TABLE ? b.p.heads : 0);

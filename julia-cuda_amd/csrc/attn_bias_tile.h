@@ -124,9 +124,10 @@ __device__ __forceinline__ KeyRange key_range(const BiasParams& p, int i) {
         const int2 s = *(const int2*)(p.span + 2 * (size_t)i);
         lo = max(s.x, 0), hi = min(s.y, p.nk);
     }
-    if (p.window > 0) {  // (positions and windows are below 2^30)
+    if (p.window > 0) {  // (pos + window may pass 2^31)
         const int pos = p.q_first + i;
-        lo = max(lo, pos - p.window), hi = min(hi, pos + p.window + 1);
+        lo = max(lo, pos - p.window);
+        hi = (int)min((uint32_t)max(hi, 0), (uint32_t)pos + (uint32_t)p.window + 1);
     }
     return hi > lo ? KeyRange{lo, hi} : KeyRange{0, 0};
 }

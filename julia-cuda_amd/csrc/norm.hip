@@ -357,9 +357,9 @@ void run(const NormParams& p, bool back, int blocks, hipStream_t st) {
     if (back) {
         const int threads = LR == 256 ? 256 : 512;
         const size_t lds = std::max<size_t>((size_t)(LR == 256 ? 1 : 8) * 2 * p.d * 4, threads * 4);
-        static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(norm_back_kernel<T, E, VEC, LR, NC>),
-                                                   hipFuncAttributeMaxDynamicSharedMemorySize, 8 * 2 * 2048 * 4) == hipSuccess;
-        if (!ok) fail("the kernel cannot have its LDS");
+        static std::atomic<uint64_t> devices{0};
+        if (!dynamic_lds(devices, reinterpret_cast<const void*>(norm_back_kernel<T, E, VEC, LR, NC>), 8 * 2 * 2048 * 4))
+            fail("the kernel cannot have its LDS");
         hipLaunchKernelGGL((norm_back_kernel<T, E, VEC, LR, NC>), dim3(blocks), dim3(threads), lds, st, p, blocks <= NORM_ONE_LAUNCH);
         return;
     }

@@ -249,6 +249,42 @@ def test_masked_infinities_and_nan_stay_where_they_are(torch_cuda, R, type):
     assert not bool(torch.isfinite(A.o[70:130, 64:]).all(1).any())
 
 
+def test_a_window_and_a_position_past_31_bits(torch_cuda, R):
+    """Positions and a window of almost 2^30: row i sees the keys from i on."""
+    say("far window")
+    far = (1 << 30) - 1
+    A = Attention(torch_cuda, R, "f16", 3, 10, heads=2, window=far, seed=23)
+    A.kw["q_first"] = far
+    A.args = lambda save=True, args=A.args: setattr_(args(save), "q_first", far)
+    A.check()
+
+
+def setattr_(a, name, value):
+    setattr(a, name, value)
+    return a
+
+
+def test_no_keys_and_no_queries(torch_cuda, R):
+    """Without keys every row is one that sees none; without queries the gradients of keys and table are 0."""
+    torch = torch_cuda
+    say("no keys")
+    A = Attention(torch, R, "f16", 40, heads=2, bias="table", seed=24)
+    A.nk = 0
+    A.forward()
+    A.backward()
+    assert bool((A.o[:40] == 0).all()) and bool((A.lse[:-1] == -math.inf).all())
+    assert bool((A.dqkv[:40, : 2 * 64] == 0).all()) and bool((A.dtable == 0).all())
+    assert bool((A.dqkv[:, 2 * 64:] == 777.0).all())
+    say("no queries")
+    A = Attention(torch, R, "f16", 40, heads=2, bias="table", seed=24)
+    A.nq, A.first = 0, 0
+    A.forward()
+    A.backward()
+    assert bool((A.o == 777.0).all()) and bool((A.lse == 777.0).all())
+    assert bool((A.dqkv[:40, 2 * 64:] == 0).all()) and bool((A.dtable == 0).all())
+    assert bool((A.dqkv[:, : 2 * 64] == 777.0).all()) and bool((A.dqkv[40:] == 777.0).all())
+
+
 @pytest.mark.parametrize("type,bias,cap,n,window", [("f16", "table", 0.0, 700, 40), ("bf16", "slopes", 20.0, 700, 0),
                                                     ("f16", "none", 0.0, 2500, 150), ("bf16", "table", 5.0, 2500, 0)])
 def test_nan_in_one_key_reaches_the_rows_that_see_it_alone(torch_cuda, R, type, bias, cap, n, window):

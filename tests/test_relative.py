@@ -79,7 +79,7 @@ REFUSED = [(dict(nq=-1), "queries"), (dict(nk=1 << 30), "keys"), (dict(heads=0, 
            (dict(q=0), "q must"), (dict(k=4098), "k must"), (dict(v=0), "v must"), (dict(o=4104), "o must"),
            (dict(q_stride=255), "apart"), (dict(q_stride=260), "apart"), (dict(kv_stride=120), "apart"),
            (dict(o_stride=1 << 23), "apart"), (dict(lse=2), "lse"),
-           (dict(nq=1 << 24, heads=256, kv_heads=256), "rows")]
+           (dict(nq=1 << 24, heads=256, kv_heads=256), "rows"), (dict(nk=1 << 29, heads=4, kv_heads=4), "keys of heads")]
 
 
 @pytest.mark.parametrize("kw,why", REFUSED, ids=[str(k) for k, _ in REFUSED])
