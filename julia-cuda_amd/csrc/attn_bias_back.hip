@@ -24,7 +24,10 @@
 //   in LDS that no other lane group adds to (64 documents in 18752 rows: dQ alone 61 us; with the sums
 //   on masked additions 128, the groups joined by shifts and an MFMA with ones 110, so 104).
 // - A block whose sums are not finite is computed again, its tiles with masked pairs pair by pair: a
-//   masked infinity or NaN times a weight of 0 is NaN in the tiles' products.
+//   masked infinity or NaN times a weight of 0 is NaN in the tiles' products. Twice the time at most.
+//
+// Both launches are bound by vector instructions and LDS reads between the products, at two (dK, dV) and
+// three (dQ) waves a SIMD: 64 documents in 18752 rows take 207 us for 44 GFLOP and 231 MB.
 #include <algorithm>
 #include <stdexcept>
 #include <string>
@@ -398,6 +401,7 @@ __global__ __launch_bounds__(64 * NW * KS) void attn_bias_dq_kernel(BiasBack b) 
 }
 
 // ---- dK and dV of 16 NG NW keys -----------------------------------------------------------------
+// (Two waves a SIMD for the blocks of one group: without the bound the compiler took registers for one.)
 template <bool BF, int BIAS, bool CAP, int NG, int NW, int KS>
 __global__ __launch_bounds__(64 * NW * KS, KS == 1 ? 2 : 1) void attn_bias_dkv_kernel(BiasBack b) {
     const BiasParams& p = b.p;
