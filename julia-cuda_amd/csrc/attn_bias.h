@@ -1,6 +1,6 @@
 // Attention whose scores may be capped by a tanh, get a bias that depends on the distance and are
 // masked by a range of keys a query, with its gradients: what the host and the kernels share
-// (attn_bias.hip: forward; attn_bias_back.hip: backward). Heads of 64, f16 or bf16.
+// (attn_bias.hip: forward; attn_bias_back.h: backward). Heads of 64, f16 or bf16.
 //
 //   s_ij = a_ij + b(j - pos_i),  a_ij = scale q_i . k_j, or cap tanh(scale q_i . k_j / cap)
 //   o_i  = sum_j exp(s_ij - lse_i) v_j over the keys that query i sees, lse_i = log sum_j exp(s_ij)
