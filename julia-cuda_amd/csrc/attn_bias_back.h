@@ -22,7 +22,7 @@
 //   to one sum; else the 16 queries of a wave are summed along the diagonals with lane shifts (a
 //   lane's four keys of a 16-key tile against its neighbours' queries) and added to rows of distances
 //   in LDS that no other lane group adds to (64 documents in 18752 rows: dQ alone 61 us; with the sums
-//   on masked additions 128, the groups joined by shifts and an MFMA with ones 110, so 104).
+//   on masked additions 128, the groups joined by shifts and an MFMA with ones 110, so 98 to 104).
 // - A block whose sums are not finite is computed again, its tiles with masked pairs pair by pair: a
 //   masked infinity or NaN times a weight of 0 is NaN in the tiles' products. Twice the time at most.
 //
